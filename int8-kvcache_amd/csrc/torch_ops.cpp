@@ -1,6 +1,8 @@
 // Thin torch extension over the C ABI of libint8kv.so (include/int8kv.h): the drop-in operators
-// int8_paged_attention, bf16_paged_attention and int8_kv_cache_write called from Python with one
-// pybind11 call each, instead of a Python wrapper plus a ctypes call of ~30 marshalled arguments.
+// int8_paged_attention, bf16_paged_attention and int8_kv_cache_write, and a serving step's
+// build_batch_tables, lora_add and sample_tokens (serving_ops.h), called from Python
+// with one pybind11 call each, instead of a Python wrapper plus a ctypes call of ~30 marshalled
+// arguments.
 //
 // What it does per call, and nothing else: the reference's argument checks (raising the same
 // exception types: AssertionError for the asserts of src/triton_ops/int8_paged_attention.py:
@@ -12,6 +14,7 @@
 
 #include <torch/extension.h>
 
+#include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
 
 #include <cmath>
@@ -20,6 +23,7 @@
 #include <utility>
 
 #include "int8kv.h"
+#include "serving_ops.h"
 
 namespace {
 
@@ -292,6 +296,141 @@ at::Tensor paged_decode(const at::Tensor& query, const at::Tensor& key_cache,
                      num_ranges, flags, workspace, min_tiles);
 }
 
+// int8kv/batch_tables.py (the same checks).
+void build_batch_tables(at::Tensor computed_lens, at::Tensor new_lens, const at::Tensor& block_tables,
+                        at::Tensor free_blocks, int64_t num_tokens, int64_t block_size,
+                        const c10::optional<at::Tensor>& free_start, const at::Tensor& query_starts,
+                        const at::Tensor& seq_lens, const at::Tensor& positions,
+                        const at::Tensor& slot_mapping, const at::Tensor& token_requests,
+                        const at::Tensor& free_end) {
+  require(computed_lens.dim() == 1 && new_lens.sizes() == computed_lens.sizes());
+  require(is_index(computed_lens.scalar_type()) &&
+          new_lens.scalar_type() == computed_lens.scalar_type());
+  const int64_t requests = computed_lens.numel();
+  require(block_tables.dim() == 2 && block_tables.size(0) == requests);
+  require(block_tables.scalar_type() == at::kInt);
+  require(block_tables.stride(1) == 1 || block_tables.size(1) <= 1 || requests == 0);
+  require(block_tables.stride(0) >= block_tables.size(1) || requests <= 1,
+          "rows of block_tables overlap");
+  require(free_blocks.dim() == 1 && free_blocks.scalar_type() == at::kInt);
+  require(num_tokens >= 0 && num_tokens <= 0x7fffffff, "num_tokens must lie in [0, 2^31 - 1]");
+  require(block_size >= 1 && block_size <= 65536, "block_size must lie in [1, 65536]");
+  require(computed_lens.is_cuda(), "build_batch_tables needs GPU tensors");
+  if (free_start.has_value()) {
+    require(free_start->scalar_type() == at::kLong && free_start->numel() == 1);
+    require_same_device({&*free_start}, computed_lens);
+  }
+  const auto buffer = [&](const at::Tensor& t, at::ScalarType type, int64_t n) {
+    require(t.scalar_type() == type && t.is_contiguous() && t.numel() == n);
+  };
+  buffer(query_starts, at::kInt, requests + 1);
+  buffer(seq_lens, at::kInt, requests);
+  buffer(positions, at::kLong, num_tokens);
+  buffer(slot_mapping, at::kLong, num_tokens);
+  buffer(token_requests, at::kInt, num_tokens);
+  buffer(free_end, at::kLong, 1);
+  require_same_device({&new_lens, &block_tables, &free_blocks, &query_starts, &seq_lens, &positions,
+                       &slot_mapping, &token_requests, &free_end},
+                      computed_lens);
+  computed_lens = computed_lens.contiguous();
+  new_lens = new_lens.contiguous();
+  free_blocks = free_blocks.contiguous();
+  const c10::hip::HIPGuard guard(computed_lens.device().index());
+  const hipStream_t stream = current_stream(computed_lens);
+  const at::Tensor ws =
+      workspace_for(computed_lens, stream, int8kv_batch_tables_workspace_bytes(requests));
+  const int st = int8kv_batch_tables(
+      computed_lens.data_ptr(), new_lens.data_ptr(), dtype_code(computed_lens.scalar_type()),
+      requests, block_tables.data_ptr<int32_t>(), block_tables.size(1), block_tables.stride(0),
+      (int32_t)block_size, free_blocks.data_ptr<int32_t>(), free_blocks.numel(),
+      free_start.has_value() ? free_start->data_ptr<int64_t>() : nullptr, num_tokens,
+      query_starts.data_ptr<int32_t>(), seq_lens.data_ptr<int32_t>(), positions.data_ptr<int64_t>(),
+      slot_mapping.data_ptr<int64_t>(), token_requests.data_ptr<int32_t>(),
+      free_end.data_ptr<int64_t>(), ws.data_ptr(), (size_t)ws.numel(), stream);
+  check_status(st, "int8kv_batch_tables");
+}
+
+// int8kv/lora.py (the same checks).
+at::Tensor lora_add(const at::Tensor& base, const at::Tensor& x, const at::Tensor& lora_a,
+                    const at::Tensor& lora_b, const at::Tensor& plan, int64_t plan_tokens,
+                    int64_t plan_adapters, c10::optional<at::Tensor> scales,
+                    c10::optional<at::Tensor> out) {
+  const auto matrix = [&](const at::Tensor& t, int64_t dim) {
+    require(t.dim() == dim && t.scalar_type() == at::kBFloat16, "lora_add takes bf16 matrices");
+    require(t.stride(-1) == 1, "lora_add takes matrices with a unit inner stride");
+  };
+  matrix(base, 2);
+  matrix(x, 2);
+  matrix(lora_a, 3);
+  matrix(lora_b, 3);
+  const int64_t tokens = x.size(0), k = x.size(1), n = base.size(1);
+  const int64_t adapters = lora_a.size(0), rank = lora_a.size(1);
+  require(base.size(0) == tokens && lora_a.size(2) == k);
+  require(lora_b.size(0) == adapters && lora_b.size(1) == n && lora_b.size(2) == rank);
+  require(k % 8 == 0 && n % 8 == 0 && rank % 8 == 0 && rank >= 8 && rank <= 128 && k > 0 && n > 0,
+          "k, n and rank must be multiples of 8, rank at most 128");
+  require(plan_tokens == tokens && plan_adapters == adapters, "a plan of other sizes");
+  require(x.is_cuda(), "lora_add needs GPU tensors");
+  if (scales.has_value()) {
+    require(scales->scalar_type() == at::kFloat && scales->dim() == 1 && scales->numel() == adapters);
+    require_same_device({&*scales}, x);
+    scales = scales->contiguous();
+  }
+  if (!out.has_value()) out = at::empty({tokens, n}, base.options());
+  require(out->sizes() == base.sizes() && out->scalar_type() == at::kBFloat16 && out->stride(1) == 1);
+  require_same_device({&base, &lora_a, &lora_b, &plan, &*out}, x);
+  const c10::hip::HIPGuard guard(x.device().index());
+  const hipStream_t stream = current_stream(x);
+  const at::Tensor ws = workspace_for(
+      x, stream, int8kv_lora_workspace_bytes(tokens, (int32_t)adapters, k, (int32_t)rank));
+  const int st = int8kv_lora_add(
+      base.data_ptr(), base.stride(0), x.data_ptr(), tokens, k, x.stride(0), lora_a.data_ptr(),
+      lora_a.strides().data(), lora_b.data_ptr(), lora_b.strides().data(), (int32_t)adapters,
+      (int32_t)rank, n, scales.has_value() ? scales->data_ptr<float>() : nullptr, plan.data_ptr(),
+      (size_t)plan.numel(), out->data_ptr(), out->stride(0), ws.data_ptr(), (size_t)ws.numel(),
+      stream);
+  check_status(st, "int8kv_lora_add");
+  return *out;
+}
+
+// int8kv/sampling.py (the same checks).
+at::Tensor sample_tokens(const at::Tensor& logits, const at::Tensor& uniforms,
+                         const c10::optional<at::Tensor>& temperature,
+                         const c10::optional<at::Tensor>& top_k,
+                         const c10::optional<at::Tensor>& top_p,
+                         const c10::optional<at::Tensor>& min_p, c10::optional<at::Tensor> out) {
+  require(logits.dim() == 2 && is_float_source(logits.scalar_type()));
+  const int64_t rows = logits.size(0), vocab = logits.size(1);
+  require(vocab >= 1 && vocab <= (1 << 22), "vocab must lie in [1, 2^22]");
+  require(logits.stride(1) == 1 || vocab == 1);
+  require(logits.stride(0) >= vocab || rows <= 1, "rows of logits overlap");
+  require(logits.is_cuda(), "sample_tokens needs GPU tensors");
+  const auto setting = [&](const c10::optional<at::Tensor>& t, at::ScalarType type) {
+    if (!t.has_value()) return at::Tensor();
+    require(t->scalar_type() == type && t->dim() == 1 && t->numel() == rows);
+    require_same_device({&*t}, logits);
+    return t->contiguous();
+  };
+  const at::Tensor u = setting(uniforms, at::kFloat), te = setting(temperature, at::kFloat),
+                   tk = setting(top_k, at::kInt), tp = setting(top_p, at::kFloat),
+                   mp = setting(min_p, at::kFloat);
+  if (!out.has_value()) out = at::empty({rows}, logits.options().dtype(at::kLong));
+  require(out->scalar_type() == at::kLong && out->is_contiguous() && out->dim() == 1 &&
+          out->numel() == rows);
+  require_same_device({&*out}, logits);
+  const c10::hip::HIPGuard guard(logits.device().index());
+  const hipStream_t stream = current_stream(logits);
+  const at::Tensor ws = workspace_for(logits, stream, int8kv_sample_workspace_bytes(rows, vocab));
+  const auto f32 = [](const at::Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; };
+  const int st = int8kv_sample_rows(
+      logits.data_ptr(), dtype_code(logits.scalar_type()), rows, vocab,
+      std::max<int64_t>(logits.stride(0), vocab), f32(u), f32(te),
+      tk.defined() ? tk.data_ptr<int32_t>() : nullptr, f32(tp), f32(mp), out->data_ptr<int64_t>(),
+      ws.data_ptr(), (size_t)ws.numel(), stream);
+  check_status(st, "int8kv_sample_rows");
+  return *out;
+}
+
 void set_library_error(py::object cls) {
   cls.inc_ref();  // kept for the life of the process
   g_library_error = cls.ptr();
@@ -323,5 +462,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("value_cache"), py::arg("block_tables"), py::arg("seq_lens"), py::arg("k_scale"),
         py::arg("v_scale"), py::arg("out"), py::arg("num_ranges"), py::arg("flags"),
         py::arg("workspace"), py::arg("min_tiles"));
+  m.def("build_batch_tables", &build_batch_tables);
+  m.def("lora_add", &lora_add);
+  m.def("sample_tokens", &sample_tokens);
   m.def("set_library_error", &set_library_error);
 }

@@ -28,7 +28,7 @@ SOURCES = ["cache_write.hip", "paged_decode.hip", "paged_decode_int8.hip", "page
            "paged_decode_fp16_pad.hip", "paged_decode_wide_int8.hip",
            "paged_decode_wide_int8_pad.hip", "paged_decode_wide_bf16.hip",
            "paged_decode_wide_fp16.hip", "decode_loop_ops.hip", "skinny_linear.hip",
-           "read_probe.hip"]
+           "batch_tables.hip", "lora.hip", "sampling.hip", "read_probe.hip"]
 # The torch extension over the C ABI (host code only; torch headers, linked to libint8kv.so).
 EXT_SOURCE = "torch_ops.cpp"
 EXT_NAME = "_int8kv_torch"

@@ -135,6 +135,31 @@ def bind(path: Path) -> ctypes.CDLL:
     ]
     lib.int8kv_argmax_rows.restype = ctypes.c_int
     lib.int8kv_argmax_rows.argtypes = [_vp, i64, i64, i64, _vp, _vp]
+    # csrc/serving_ops.h (batch_tables.py, lora.py, sampling.py)
+    lib.int8kv_batch_tables_workspace_bytes.restype = sz
+    lib.int8kv_batch_tables_workspace_bytes.argtypes = [i64]
+    lib.int8kv_batch_tables.restype = ctypes.c_int
+    lib.int8kv_batch_tables.argtypes = [
+        _vp, _vp, ctypes.c_int, i64, _vp, i64, i64, i32, _vp, i64, _vp, i64, _vp, _vp, _vp, _vp, _vp,
+        _vp, _vp, sz, _vp,
+    ]
+    lib.int8kv_lora_plan_bytes.restype = sz
+    lib.int8kv_lora_plan_bytes.argtypes = [i64, i32]
+    lib.int8kv_lora_plan.restype = ctypes.c_int
+    lib.int8kv_lora_plan.argtypes = [_vp, ctypes.c_int, i64, i32, _vp, sz, _vp]
+    lib.int8kv_lora_workspace_bytes.restype = sz
+    lib.int8kv_lora_workspace_bytes.argtypes = [i64, i32, i64, i32]
+    lib.int8kv_lora_add.restype = ctypes.c_int
+    lib.int8kv_lora_add.argtypes = [
+        _vp, i64, _vp, i64, i64, i64, _vp, _c_i64p, _vp, _c_i64p, i32, i32, i64, _vp, _vp, sz, _vp,
+        i64, _vp, sz, _vp,
+    ]
+    lib.int8kv_sample_workspace_bytes.restype = sz
+    lib.int8kv_sample_workspace_bytes.argtypes = [i64, i64]
+    lib.int8kv_sample_rows.restype = ctypes.c_int
+    lib.int8kv_sample_rows.argtypes = [
+        _vp, ctypes.c_int, i64, i64, i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, sz, _vp,
+    ]
     # csrc/skinny_linear.h (the decode loop's own products, not part of the public C ABI)
     lib.int8kv_skinny_linear_ok.restype = i32
     lib.int8kv_skinny_linear_ok.argtypes = [i64, i64, i64]

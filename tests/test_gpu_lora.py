@@ -1,0 +1,198 @@
+"""lora_plan and lora_add against 64 bits, within the bound that fp32 sums, the two bf16 parts of the
+rank-wide vector and one rounding to bf16 allow (serving_cases.lora_ref derives it)."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import int8kv
+from int8kv import _ext, _lib
+from serving_cases import lora_ref
+
+pytestmark = pytest.mark.gpu
+
+
+def inputs(cuda, tokens, k, n, rank, adapters, seed, ids=None):
+    g = torch.Generator().manual_seed(seed)
+
+    def normal(*size, std=1.0):
+        return (torch.randn(*size, generator=g) * std).to(torch.bfloat16)
+
+    if ids is None:
+        ids = torch.randint(-1, adapters, (tokens,), generator=g)
+    d = dict(base=normal(tokens, n), x=normal(tokens, k), a=normal(adapters, rank, k, std=k**-0.5),
+             b=normal(adapters, n, rank, std=0.1), scales=torch.rand(adapters, generator=g) * 3 - 1)
+    d = {key: t.to(cuda) for key, t in d.items()}
+    d["ids"] = ids.to(cuda)
+    return d
+
+
+def check(d, out, scales=True):
+    f = {key: d[key].float().cpu().numpy() for key in ("base", "x", "a", "b", "scales")}
+    s = f["scales"] if scales else np.ones_like(f["scales"])
+    ref, bound = lora_ref(f["base"], f["x"], f["a"], f["b"], d["ids"].cpu().tolist(),
+                          s.astype(np.float64))
+    off = np.abs(out.float().cpu().numpy().astype(np.float64) - ref)
+    assert (off <= bound).all(), float((off - bound).max())
+
+
+def add(d, **kw):
+    plan = int8kv.lora_plan(d["ids"], d["a"].shape[0])
+    kw.setdefault("scales", d["scales"])
+    return int8kv.lora_add(d["base"], d["x"], d["a"], d["b"], plan, **kw)
+
+
+@pytest.mark.parametrize("tokens,k,n,rank,adapters", [
+    (1, 8, 8, 8, 1),
+    (1, 3584, 4608, 16, 8),
+    (5, 264, 136, 24, 3),
+    (17, 512, 1000, 8, 40),
+    (32, 3584, 520, 16, 24),
+    (33, 1032, 264, 40, 4),
+    (64, 128, 72, 64, 2),
+    (100, 640, 392, 72, 5),
+    (130, 256, 264, 128, 7),
+    (200, 40, 16, 120, 200),
+    (700, 520, 328, 32, 9),
+    (1030, 264, 520, 104, 3),
+])
+def test_against_64_bits(cuda, tokens, k, n, rank, adapters):
+    d = inputs(cuda, tokens, k, n, rank, adapters, seed=tokens + k)
+    check(d, add(d))
+    check(d, add(d, scales=None), scales=False)
+
+
+def test_runs_of_one_adapter_and_none(cuda):
+    """Prefill-like runs, all tokens on one adapter, and no token with one."""
+    ids = torch.repeat_interleave(torch.tensor([2, -1, 0, 3, 2, 1]), torch.tensor([70, 9, 1, 150, 64, 33]))
+    d = inputs(cuda, 327, 264, 136, 16, 4, seed=1, ids=ids)
+    check(d, add(d))
+    d["ids"] = torch.full((327,), 1, device=cuda)
+    check(d, add(d))
+    for none in (-1, -(2**31), 4, 2**31 - 1):
+        d["ids"] = torch.full((327,), none, device=cuda, dtype=torch.int32)
+        assert torch.equal(add(d), d["base"])
+
+
+def test_rows_without_an_adapter_are_the_base_rows(cuda):
+    """Bit for bit, NaN and infinities included; the other rows are not touched by them."""
+    d = inputs(cuda, 40, 128, 64, 16, 3, seed=2)
+    none = d["ids"] < 0
+    clean = add(d)
+    d["base"][none] = float("nan")
+    d["x"][none] = float("inf")
+    out = add(d)
+    assert torch.isnan(out[none]).all() and torch.equal(out[~none], clean[~none])
+
+
+def test_non_finite_rows_stay_their_own(cuda):
+    """One token's infinity reaches its own row alone, also among tokens of the same adapter."""
+    d = inputs(cuda, 50, 264, 72, 16, 2, seed=3, ids=torch.arange(50) % 2)
+    clean = add(d)
+    d["x"][7, 5] = float("inf")
+    out = add(d)
+    keep = torch.arange(50, device=cuda) != 7
+    assert torch.equal(out[keep], clean[keep]) and not torch.isfinite(out[7]).any()
+
+
+def test_infinite_intermediate_without_sign_conflict(cuda):
+    """x A^T infinite and B of one sign: the sum is that infinity, as in plain arithmetic."""
+    d = inputs(cuda, 3, 64, 16, 8, 1, seed=4, ids=torch.zeros(3, dtype=torch.int64))
+    d["x"].fill_(3.0e38)
+    d["a"].fill_(1.0)
+    d["b"].fill_(0.5)
+    d["scales"].fill_(1.0)
+    assert (add(d) == float("inf")).all()
+
+
+def test_large_intermediate_keeps_its_bits(cuda):
+    """A rank-wide vector close to the largest fp32 value: its upper part must not overflow."""
+    d = inputs(cuda, 2, 64, 16, 8, 1, seed=5, ids=torch.zeros(2, dtype=torch.int64))
+    d["x"].zero_()
+    d["x"][:, 0] = 3.3895e38  # the largest bf16 value
+    d["a"].zero_()
+    d["a"][0, 0, 0] = 1.0
+    d["b"].zero_()
+    d["b"][0, :, 0] = 2.0**-100
+    d["scales"].fill_(1.0)
+    out = add(d).float()
+    want = d["base"].float() + d["x"][0, 0].float() * 2.0**-100
+    assert torch.allclose(out, want, rtol=2.0**-8, atol=0)
+
+
+def test_views_and_in_place(cuda):
+    """Base and out inside wider rows (a slice of a packed projection), weights inside wider
+    buffers, int64 ids, out in place; the columns around stay."""
+    d = inputs(cuda, 37, 264, 136, 24, 5, seed=6)
+    want = add(d)
+    packed = torch.full((37, 400), 7.0, dtype=torch.bfloat16, device=cuda)
+    packed[:, 64:200] = d["base"]
+    view = packed[:, 64:200]
+    xs = torch.zeros(37, 512, dtype=torch.bfloat16, device=cuda)
+    xs[:, 16:280] = d["x"]
+    aw = torch.zeros(5, 32, 512, dtype=torch.bfloat16, device=cuda)
+    aw[:, 8:, 8:272] = d["a"]
+    bw = torch.zeros(5, 200, 64, dtype=torch.bfloat16, device=cuda)
+    bw[:, 3:139, 16:40] = d["b"]
+    plan = int8kv.lora_plan(d["ids"].long(), 5)
+    got = int8kv.lora_add(view, xs[:, 16:280], aw[:, 8:, 8:272], bw[:, 3:139, 16:40], plan,
+                          scales=d["scales"], out=view)
+    assert got.data_ptr() == view.data_ptr() and torch.equal(view, want)
+    assert (packed[:, :64] == 7).all() and (packed[:, 200:] == 7).all()
+
+
+def test_ctypes_path_and_other_stream(cuda):
+    d = inputs(cuda, 90, 520, 264, 32, 6, seed=7)
+    want = add(d)
+    side = torch.cuda.Stream(cuda)
+    side.wait_stream(torch.cuda.current_stream(cuda))
+    with torch.cuda.stream(side):
+        got = add(d)
+    side.synchronize()
+    with _ext.use_ctypes():
+        other = add(d)
+    assert torch.equal(got, want) and torch.equal(other, want)
+
+
+def test_repeated_calls_are_bit_identical(cuda):
+    d = inputs(cuda, 600, 1032, 264, 16, 30, seed=8)
+    want = add(d)
+    for _ in range(3):
+        assert torch.equal(add(d), want)
+
+
+def test_captured_plan_follows_the_ids(cuda):
+    """Plan and product captured; the ids change between replays, with eager calls in between."""
+    d = inputs(cuda, 24, 264, 136, 16, 6, seed=9)
+    other = inputs(cuda, 300, 520, 264, 64, 6, seed=10)
+    out = torch.empty_like(d["base"])
+    plan = int8kv.lora_plan(d["ids"], 6)
+    int8kv.lora_add(d["base"], d["x"], d["a"], d["b"], plan, scales=d["scales"], out=out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        int8kv.lora_plan(d["ids"], 6, plan=plan)
+        int8kv.lora_add(d["base"], d["x"], d["a"], d["b"], plan, scales=d["scales"], out=out)
+    for step in range(4):
+        d["ids"].copy_(torch.randint(-1, 6, (24,), generator=torch.Generator().manual_seed(step)))
+        graph.replay()
+        check(other, add(other))
+        torch.cuda.synchronize()
+        check(d, out)
+
+
+def test_no_tokens(cuda):
+    d = inputs(cuda, 0, 64, 16, 8, 2, seed=11)
+    assert add(d).shape == (0, 16)
+
+
+def test_misaligned_rows_are_refused(cuda):
+    d = inputs(cuda, 4, 64, 16, 8, 2, seed=12)
+    plan = int8kv.lora_plan(d["ids"], 2)
+    wide = torch.zeros(4, 73, dtype=torch.bfloat16, device=cuda)
+    with pytest.raises(_lib.Int8KVError, match="STRIDE"):
+        int8kv.lora_add(d["base"], wide[:, 1:65], d["a"], d["b"], plan)
+    with pytest.raises(AssertionError):
+        int8kv.lora_add(d["base"][:, ::2], d["x"], d["a"], d["b"], plan)
