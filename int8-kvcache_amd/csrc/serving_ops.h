@@ -107,12 +107,12 @@ int int8kv_lora_add(const void* base, int64_t base_row_stride, const void* x, in
  * all kept weights (uniforms below 0 or NaN count as 0, from 1 on as the largest number below 1).
  * Rows with T <= 0 (or NaN), or whose logits are all -inf or NaN, give the first maximum of v.
  *
- * Weights are rounded to multiples of 2^-40 or finer (2^-44 at vocab 152064), computed in 64 bits,
+ * Weights are rounded to multiples of 2^-41 or finer (2^-44 at vocab 152064), computed in 64 bits,
  * and summed as integers, so that a row's token depends on nothing but its inputs.
  *
  *   uniforms: fp32 [rows]; temperature, top_p, min_p: fp32 [rows] or NULL (1, 1, 0); top_k: int32
  *   [rows] or NULL (0); all contiguous.
- *   vocab in [1, 2^22].  out: int64 [rows].
+ *   vocab in [1, 2^21], rows at most 2^16.  out: int64 [rows].
  *   workspace: int8kv_sample_workspace_bytes(rows, vocab) bytes, 16-byte aligned, no
  *   initialisation needed; calls that share one must not overlap.
  */

@@ -401,7 +401,8 @@ at::Tensor sample_tokens(const at::Tensor& logits, const at::Tensor& uniforms,
                          const c10::optional<at::Tensor>& min_p, c10::optional<at::Tensor> out) {
   require(logits.dim() == 2 && is_float_source(logits.scalar_type()));
   const int64_t rows = logits.size(0), vocab = logits.size(1);
-  require(vocab >= 1 && vocab <= (1 << 22), "vocab must lie in [1, 2^22]");
+  require(vocab >= 1 && vocab <= (1 << 21), "vocab must lie in [1, 2^21]");
+  require(rows <= (1 << 16), "at most 2^16 rows");
   require(logits.stride(1) == 1 || vocab == 1);
   require(logits.stride(0) >= vocab || rows <= 1, "rows of logits overlap");
   require(logits.is_cuda(), "sample_tokens needs GPU tensors");

@@ -11,7 +11,8 @@ import torch
 
 from . import _decode, _ext, _lib
 
-MAX_VOCAB = 1 << 22
+MAX_VOCAB = 1 << 21
+MAX_ROWS = 1 << 16
 
 
 def sample_tokens(
@@ -42,7 +43,8 @@ def sample_tokens(
         return ext.sample_tokens(logits, uniforms, temperature, top_k, top_p, min_p, out)
     assert logits.dim() == 2 and logits.dtype in _decode.QUERY_DTYPES
     rows, vocab = logits.shape
-    assert 1 <= vocab <= MAX_VOCAB, "vocab must lie in [1, 2^22]"
+    assert 1 <= vocab <= MAX_VOCAB, "vocab must lie in [1, 2^21]"
+    assert rows <= MAX_ROWS, "at most 2^16 rows"
     assert logits.stride(1) == 1 or vocab == 1
     assert logits.stride(0) >= vocab or rows <= 1, "rows of logits overlap"
     assert logits.is_cuda, "sample_tokens needs GPU tensors"

@@ -128,6 +128,57 @@ def test_dense_values_at_the_cut(cuda):
             both(cuda, logits, u, **kw)
 
 
+def test_cuts_of_every_size(cuda):
+    """top-k from one token to the whole vocabulary, beside nuclei from nothing to everything: cuts
+    from piece maxima, from bins, and past both lists; masked rows with fewer tokens than top-k."""
+    g = torch.Generator().manual_seed(14)
+    ks = [1, 2, 15, 16, 17, 60, 70, 127, 128, 129, 700, 4096, 4097, 9000, 30000, 32767, 32768, 50000]
+    ps = [1.0, 0.02, 0.3, 0.7, 0.97, 0.9999, 1 - 2.0**-24]
+    for dtype in DTYPES:
+        for vocab, live in ((32768, 1.0), (32771, 0.2), (32771, 0.001)):
+            logits = torch.randn(len(ks), vocab, generator=g) * 2.5
+            logits[torch.rand(len(ks), vocab, generator=g) >= live] = -INF
+            logits[:, 77] = 1.0
+            logits = logits.to(dtype)
+            for p in ps:
+                u = torch.rand(len(ks), generator=g)
+                both(cuda, logits, u, top_k=ks, top_p=p, temperature=0.9)
+            both(cuda, logits, u, top_k=ks)  # (without top_p no histogram pass runs)
+
+
+def test_live_tokens_in_few_places(cuda):
+    """All live tokens in one corner of the row, more and fewer than the list holds."""
+    g = torch.Generator().manual_seed(15)
+    for lo, n in ((0, 300), (40000, 300), (49000, 1003), (20000, 5000), (0, 20000)):
+        logits = torch.full((6, 50003), -INF)
+        logits[:, lo:lo + n] = torch.randn(6, n, generator=g)
+        u = torch.rand(6, generator=g)
+        for kw in ({}, {"top_k": 80}, {"top_k": 80, "top_p": 0.9}, {"top_p": 0.9}, {"top_k": 2000},
+                   {"min_p": 0.2}, {"top_k": 30000, "top_p": 0.5}):
+            both(cuda, logits, u, **kw)
+
+
+def test_vocabularies_of_more_pieces_than_tiles(cuda):
+    for vocab in (262145, 400003, 2**21):
+        logits, u = random_logits(2, vocab, torch.bfloat16, seed=vocab)
+        for kw in ({}, {"top_k": 50}, {"top_p": 0.9}, {"top_k": 5000, "top_p": 0.9, "min_p": 0.01},
+                   {"min_p": 0.1}, {"temperature": 0.0}):
+            both(cuda, logits, u, **kw)
+
+
+def test_far_and_near_chunks(cuda):
+    """Chunks whose maxima lie far below the row's, and equal ones: the plain path's scaling."""
+    g = torch.Generator().manual_seed(16)
+    logits = torch.randn(64, 40000, generator=g)
+    logits += torch.repeat_interleave(torch.tensor([-30.0, 0.0, -3.0, -80.0, -0.5]), 8000)
+    both(cuda, logits, torch.rand(64, generator=g))
+    both(cuda, logits, torch.rand(64, generator=g), temperature=5.0)
+    both(cuda, logits, torch.rand(64, generator=g), temperature=0.1)
+    low = torch.full((1, 40000), -1e4)
+    low[0, 39999] = 3.0
+    assert run(cuda, low.expand(2, -1).contiguous(), [0.0, 1 - 2.0**-24]) == [39999, 39999]
+
+
 def test_masks(cuda):
     """Tokens at -inf, at the type's lowest value and at NaN: never drawn while another is left;
     one token left; none left."""

@@ -98,14 +98,14 @@ def test_sample_refusals(lib):
     for name in ("logits", "u", "out"):
         assert call(**{name: None}) == -1, name
     assert call(dt=3) == -2 and call(dt=4) == -2
-    for bad in (dict(rows=-1), dict(rows=2**31), dict(vocab=0), dict(vocab=2**22 + 1, rs=2**23)):
+    for bad in (dict(rows=-1), dict(rows=2**16 + 1), dict(vocab=0), dict(vocab=2**21 + 1, rs=2**23)):
         assert call(**bad) == -3, bad
     assert call(rs=99) == -4 and call(logits=17) == -4 and call(dt=0, logits=18) == -4
     assert call(ws=None) == -5 and call(wsb=8) == -5 and call(ws=24) == -5
     assert call(rows=0) == 0
     assert lib.int8kv_sample_workspace_bytes(4, 0) == 0
     assert lib.int8kv_sample_workspace_bytes(-1, 100) == 0
-    assert lib.int8kv_sample_workspace_bytes(4, 2**22 + 1) == 0
+    assert lib.int8kv_sample_workspace_bytes(4, 2**21 + 1) == 0
 
 
 def test_python_entry_points_refuse(path):
