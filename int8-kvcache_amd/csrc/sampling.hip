@@ -49,14 +49,17 @@ struct SampleArgs {
   const float* top_p;
   const float* min_p;
   int64_t* out;
-  int32_t chunks;   // of the first pass, per row
+  int32_t chunks;   // of the first pass, per row, taken in `runs` of `run_chunks`
+  int32_t runs, run_chunks;
   int32_t pieces;   // kChunkElements / kPieceElements of each chunk
   int32_t parts;    // workgroups per row of the histogram pass (0: it does not run)
   float* chunk_max;      // [rows][chunks]
   uint64_t* chunk_mass;  // [rows][chunks] (rows without a filter), in units of the chunk's own maximum
   float* piece_max;      // [rows][pieces]
   uint64_t* bin_mass;    // [rows][kBins]
-  uint32_t* bin_count;   // [rows][kBins]
+  uint64_t* tile_mass;   // [rows][kMaxTiles]
+  uint64_t* list;        // [rows][kList] places
+  int32_t* list_count;   // [rows] tokens of the list
 };
 
 // ------------------------------------------------------------------------------ row access
@@ -64,17 +67,20 @@ struct SampleArgs {
 // vectors, the last slot what is left.  Elements a slot lacks read as -inf (weight 0).
 template <int DT>
 struct Row {
-  static constexpr int kE = DT == kF32 ? 4 : 8;  // elements of a vector
+  static constexpr int kE = DT == kF32 ? 4 : 8;     // elements of a vector
+  static constexpr int kSize = DT == kF32 ? 4 : 2;  // bytes of one
   const char* p;
+  const u32x4* body;  // the whole vectors (any readable memory if there are none)
   int32_t vocab, head, vectors;
 
   __device__ __forceinline__ Row(const SampleArgs& a, int64_t r) {
-    constexpr int size = DT == kF32 ? 4 : 2;
-    p = static_cast<const char*>(a.logits) + r * a.row_stride * size;
+    p = static_cast<const char*>(a.logits) + r * a.row_stride * kSize;
     vocab = a.vocab;
-    const int32_t off = (int32_t)((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / size;
+    const int32_t off = (int32_t)((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / kSize;
     head = off < vocab ? off : vocab;
     vectors = (vocab - head) / kE;
+    body = vectors > 0 ? reinterpret_cast<const u32x4*>(p + (int64_t)head * kSize)
+                       : reinterpret_cast<const u32x4*>(a.chunk_mass);
   }
   __device__ __forceinline__ int32_t slots() const { return vectors + 2; }
   // Index of a slot's first element.
@@ -89,23 +95,31 @@ struct Row {
     else
       return (float)reinterpret_cast<const _Float16*>(p)[i];
   }
-  // The slot's values, NaN as -inf.
-  __device__ __forceinline__ void load(int32_t s, float (&v)[kE]) const {
-    if (s >= 1 && s <= vectors) {
-      const char* q = p + (int64_t)head * (DT == kF32 ? 4 : 2) + 16 * (int64_t)(s - 1);
-      if constexpr (DT == kF32) {
-        const f32x4 x = *reinterpret_cast<const f32x4*>(q);
+  // A slot's vector, requested without a branch (an edge slot requests a neighbour's).
+  __device__ __forceinline__ u32x4 request(int32_t s) const {
+    const int32_t i = s - 1 < vectors - 1 ? s - 1 : vectors - 1;
+    return body[i > 0 ? i : 0];
+  }
+  // The slot's values from what request() gave, NaN as it is.  INNER: no edge slot.
+  template <bool INNER>
+  __device__ __forceinline__ void values(int32_t s, u32x4 raw, float (&v)[kE]) const {
+    if constexpr (DT == kF32) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = x[j];
-      } else {
-        int8kv::load8_f32<DT>(q, v);
-      }
+      for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(raw[j]);
     } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) int8kv::unpack2<DT>(raw[j], v[2 * j], v[2 * j + 1]);
+    }
+    if (!INNER && !(s >= 1 && s <= vectors)) {
       const int32_t i0 = first(s);
       const int32_t n = s == 0 ? head : (s == vectors + 1 ? vocab - i0 : 0);
 #pragma unroll
       for (int j = 0; j < kE; ++j) v[j] = j < n ? element(i0 + j) : -INFINITY;
     }
+  }
+  // The slot's values, NaN as -inf.
+  __device__ __forceinline__ void load(int32_t s, float (&v)[kE]) const {
+    values<false>(s, request(s), v);
 #pragma unroll
     for (int j = 0; j < kE; ++j) v[j] = fmaxf(v[j], -INFINITY);  // (fmaxf: the number, if one is NaN)
   }
@@ -121,9 +135,26 @@ __device__ __forceinline__ float value_of(uint32_t key) {
 }
 
 // ---------------------------------------------------------------------------------- weights
-// w(v) = 2^((v - M) log2(e) / T) in units of 2^-frac, rounded to even.  With y = n + f, |f| <= 1/2,
-// 2^f by a polynomial (interpolation at Chebyshev nodes, relative error 4e-14, exactly 1 at f = 0)
-// and the rounding by adding 2^52: the integer is left in the low bits.
+// w(v) = 2^((v - M) log2(e) / T) in units of 2^-frac.  With y = n + f, |f| <= 1/2, 2^f by a
+// polynomial (interpolation at Chebyshev nodes, relative error 2e-12, exactly 1 at f = 0).
+__device__ __forceinline__ double exp2_part(double f) {
+  double p = 0x1.63b2d796ba66ap-20;
+  p = fma(p, f, 0x1.00c0e4e15180ap-16);
+  p = fma(p, f, 0x1.4308c7183da5dp-13);
+  p = fma(p, f, 0x1.5d877598350fdp-10);
+  p = fma(p, f, 0x1.3b2ab70ad2564p-7);
+  p = fma(p, f, 0x1.c6b08da70cce3p-5);
+  p = fma(p, f, 0x1.ebfbdff82a734p-3);
+  p = fma(p, f, 0x1.62e42fef9cc69p-1);
+  return fma(p, f, 1.0);
+}
+// 2^(frac + n), n >= -102.
+__device__ __forceinline__ double exp2_scale(int32_t n, int32_t frac) {
+  return __hiloint2double((n + (1023 + frac)) << 20, 0);
+}
+constexpr double kRound = 0x1.8p52;  // y + kRound - kRound: y rounded to an integer, left in the low bits
+
+// Rounded to integers by adding 2^52: the integer is left in the low bits.
 struct Weights {
   double c;    // log2(e) / T
   double top;  // M
@@ -131,61 +162,129 @@ struct Weights {
   int32_t frac;
 
   __device__ __forceinline__ uint64_t operator()(float v) const {
-    constexpr double kMagic = 0x1.8p52;
-    double y = ((double)v - top) * c;
-    y = v == topf ? 0.0 : fmax(y, -100.0);  // (NaN, from infinities: -100, weight 0)
-    const double t = y + kMagic;
-    const double f = y - (t - kMagic);
-    const int32_t n = (int32_t)__double_as_longlong(t);
-    double p = 0x1.b63880fccd758p-24;
-    p = fma(p, f, 0x1.63d13634289c7p-20);
-    p = fma(p, f, 0x1.ffcb951552801p-17);
-    p = fma(p, f, 0x1.4308ac85ac77dp-13);
-    p = fma(p, f, 0x1.5d87fe86fea1cp-10);
-    p = fma(p, f, 0x1.3b2ab7181b747p-7);
-    p = fma(p, f, 0x1.c6b08d7047e51p-5);
-    p = fma(p, f, 0x1.ebfbdff823cedp-3);
-    p = fma(p, f, 0x1.62e42fefa39efp-1);
-    p = fma(p, f, 1.0);
-    const double scale = __longlong_as_double((int64_t)(1023 + frac + n) << 52);
-    const double r = fma(p, scale, 0x1p52);
+    if (topf == INFINITY) return v == topf ? (uint64_t)1 << frac : 0;
+    const double y = fmax(((double)v - top) * c, -100.0);  // (NaN, of -inf and T = inf: -100, weight 0)
+    const double t = y + kRound;
+    const double p = exp2_part(y - (t - kRound));
+    const double r = fma(p, exp2_scale(__double2loint(t), frac), 0x1p52);
     return (uint64_t)__double_as_longlong(r) - 0x4330000000000000ull;
   }
 };
 
+// The same up to the last bits of y for ordinary temperatures and logits, added to a sum that
+// starts at 2^52 (at most 16 weights: below 2^53, so that each is rounded to an integer): 15
+// 64-bit operations per weight instead of 19, and no test.  A row's chunk masses and the choice
+// within the chunk both use it.
+struct FastWeights {
+  double c, k;  // y = v c - k
+  float low;    // y = -100 here
+  int32_t frac;
+
+  __device__ __forceinline__ FastWeights(float t, float top, int32_t fraction) {
+    c = 0x1.71547652b82fep+0 / (double)t;
+    k = (double)top * c;
+    low = (float)((double)top - 100.0 / c);
+    frac = fraction;
+  }
+  // The maximum's weight is exactly 2^frac, and `low` lies below the maximum.
+  static __device__ __forceinline__ bool fits(float t, float top) {
+    return t > 0x1p-10f && t < 0x1p10f && fabsf(top) < 64.0f * t;
+  }
+  __device__ __forceinline__ double add(float v, double sum) const {
+    const double y = fma((double)fmaxf(v, low), c, -k);
+    const double t = y + kRound;
+    const double p = exp2_part(y - (t - kRound));
+    return fma(p, exp2_scale(__double2loint(t), frac), sum);
+  }
+  __device__ __forceinline__ uint64_t operator()(float v) const { return value(add(v, 0x1p52)); }
+  static __device__ __forceinline__ uint64_t value(double sum) {
+    return (uint64_t)__double_as_longlong(sum) - 0x4330000000000000ull;
+  }
+};
+
 // ------------------------------------------------------------------------- workgroup sums
-__device__ __forceinline__ uint64_t wave_sum(uint64_t v) {
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor((unsigned long long)v, d, 64);
-  return v;
+// Barrier for data exchanged through LDS: loads in flight stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+// A lane's value moved along the wave without LDS (DPP): CTRL row_shr 1, 2, 4, 8 within 16 lanes,
+// row_bcast 15 and 31 across them.  Lanes without a source keep `old`.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp(uint32_t old, uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)old, (int)v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_add(uint32_t v) {
+  return v + dpp<CTRL, ROWS>(0u, v);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp_add(uint64_t v) {
+  const uint32_t lo = dpp<CTRL, ROWS>(0u, (uint32_t)v);
+  const uint32_t hi = dpp<CTRL, ROWS>(0u, (uint32_t)(v >> 32));
+  return v + (((uint64_t)hi << 32) | lo);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_max(float v) {
+  const uint32_t b = __float_as_uint(v);
+  return fmaxf(v, __uint_as_float(dpp<CTRL, ROWS>(b, b)));
 }
 // Inclusive prefix sum over the wave.
 template <typename T>
 __device__ __forceinline__ T wave_scan(T v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const T up = __shfl_up(v, d, 64);
-    if (lane >= d) v += up;
-  }
-  return v;
+  v = dpp_add<0x111, 0xf>(v);
+  v = dpp_add<0x112, 0xf>(v);
+  v = dpp_add<0x114, 0xf>(v);
+  v = dpp_add<0x118, 0xf>(v);
+  v = dpp_add<0x142, 0xa>(v);
+  return dpp_add<0x143, 0xc>(v);
+}
+// The largest (or smallest) of the lanes' values, in lane 63.
+template <bool LARGEST>
+__device__ __forceinline__ uint32_t wave_extreme(uint32_t v) {
+  const auto pick = [](uint32_t a, uint32_t b) { return (a > b) == LARGEST ? a : b; };
+  v = pick(v, dpp<0x111, 0xf>(v, v));
+  v = pick(v, dpp<0x112, 0xf>(v, v));
+  v = pick(v, dpp<0x114, 0xf>(v, v));
+  v = pick(v, dpp<0x118, 0xf>(v, v));
+  v = pick(v, dpp<0x142, 0xa>(v, v));
+  return pick(v, dpp<0x143, 0xc>(v, v));
+}
+__device__ __forceinline__ uint32_t last_lane(uint32_t v, int lane = 63) {
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+}
+__device__ __forceinline__ uint64_t last_lane(uint64_t v, int lane = 63) {
+  return ((uint64_t)last_lane((uint32_t)(v >> 32), lane) << 32) | last_lane((uint32_t)v, lane);
+}
+__device__ __forceinline__ uint64_t wave_sum(uint64_t v) { return last_lane(wave_scan(v)); }
+// Running maximum: lane 15 of each 16, then lanes 31 and 63 hold their 32 lanes', then lane 63 all.
+__device__ __forceinline__ float max_to_31(float m) {
+  m = dpp_max<0x111, 0xf>(m);
+  m = dpp_max<0x112, 0xf>(m);
+  m = dpp_max<0x114, 0xf>(m);
+  m = dpp_max<0x118, 0xf>(m);
+  return dpp_max<0x142, 0xa>(m);
+}
+__device__ __forceinline__ float max_to_63(float m) { return dpp_max<0x143, 0xc>(m); }
+__device__ __forceinline__ float wave_max(float m) {
+  return __uint_as_float(last_lane(__float_as_uint(max_to_63(max_to_31(m)))));
 }
 // Exclusive prefix sum over the workgroup; s_wave: kWaves values.
 template <typename T>
 __device__ __forceinline__ T workgroup_scan(T v, T* s_wave, T& total) {
+  static_assert(kWaves <= 16, "the waves' sums are scanned by 16 lanes");
   const int lane = threadIdx.x & 63;
-  const int wave = threadIdx.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const T inc = wave_scan(v);
   __syncthreads();
   if (lane == 63) s_wave[wave] = inc;
   __syncthreads();
-  T before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    if (w < wave) before += s_wave[w];
-    total += s_wave[w];
-  }
+  T w = s_wave[lane & (kWaves - 1)];
+  w = dpp_add<0x111, 0xf>(w);
+  w = dpp_add<0x112, 0xf>(w);
+  w = dpp_add<0x114, 0xf>(w);
+  w = dpp_add<0x118, 0xf>(w);
+  total = last_lane(w, kWaves - 1);
+  const T before = wave > 0 ? last_lane(w, wave - 1) : 0;
   return before + inc - v;
 }
 
@@ -234,112 +333,125 @@ __device__ __forceinline__ uint64_t scaled(double u, uint64_t z) {
 }
 
 // ------------------------------------------------------------------------------- histogram
-// Bins of d = M - v, 64 to an octave from 2^-10 to 256, one below and one above: fine where a
+// Bins of d = M - v, 128 to an octave from 2^-10 to 256, one below and one above: fine where a
 // cut can lie whatever the temperature, and monotone in v (the subtraction rounds monotonically).
-constexpr int kBinShift = 17;                        // 6 mantissa bits
-constexpr int kBinBase = (127 - 10) << 6;
-constexpr int kOctaveBins = 18 * 64;
-constexpr int kBins = kOctaveBins + 2;
+constexpr int kBinShift = 16;  // 7 mantissa bits
+constexpr int kBinBase = (127 - 10) << 7;
+constexpr int kBins = 18 * 128 + 2;
+constexpr int kThreadBins = (kBins + kThreads - 1) / kThreads;
 __device__ __forceinline__ int32_t bin_of(float v, float top) {
   const float d = v == top ? 0.0f : top - v;
   const int32_t b = (int32_t)(__float_as_uint(d) >> kBinShift) - kBinBase + 1;
   return b < 0 ? 0 : (b < kBins ? b : kBins - 1);
 }
 
-// Rows whose top-k cut is found from the piece maxima alone: at least half of the pieces lie
-// below the k-th largest maximum.
-__device__ __forceinline__ bool by_pieces(const SampleArgs& a, const Params& q) {
-  return q.k > 0 && q.k <= a.pieces / 2;
-}
+// Rows with a nucleus cut alone: their histogram pass and gathering run over many workgroups.  (A
+// row of at most kList tokens lists them all.)
 __device__ __forceinline__ bool needs_bins(const SampleArgs& a, const Params& q) {
-  return !q.greedy && (q.k > 0 || q.p < 1.0) && !by_pieces(a, q);
+  return a.parts > 0 && !q.greedy && q.k == 0 && q.p < 1.0;
 }
 
-template <int DT>
-__device__ __forceinline__ void add_to_bins(const Row<DT>& row, const Weights& w, const Params& q,
-                                            int32_t s0, int32_t s1, uint64_t* mass,
-                                            uint32_t* count) {
-  for (int32_t i = s0 + (int32_t)threadIdx.x; i < s1; i += kThreads) {
-    float v[Row<DT>::kE];
-    row.load(i, v);
-#pragma unroll
-    for (int j = 0; j < Row<DT>::kE; ++j)
-      if (v[j] > -INFINITY) {
-        const int32_t b = bin_of(v[j], w.topf);
-        if (q.k > 0) atomicAdd(&count[b], 1u);
-        if (q.p < 1.0)
-          atomicAdd(reinterpret_cast<unsigned long long*>(&mass[b]), (unsigned long long)w(v[j]));
-      }
-  }
-}
-
-__device__ __forceinline__ float wave_max(float m) {
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
-  return m;
-}
+// Tokens waiting for their weights, so that those are computed by whole waves: value and index.
+constexpr int kQueue = 4096;
+struct Queue {
+  float value[kQueue];
+  int32_t index[kQueue];
+  int32_t length;
+};
 
 // ------------------------------------------------------------------------------ first pass
-// One chunk of one row, held in registers: the maxima of its pieces and its own, and, for rows
-// without a filter, the sum of its weights in units of its own maximum (so that the data is read
-// once).  Clears the row's bins where they will be used.
+// A run of chunks of one row, each held in registers while the next one is loaded: the maxima of
+// their pieces and their own, and, for rows whose whole mass is needed, the sum of their weights in
+// units of their own maximum (so that the data is read once).  Clears the row's bins where they
+// will be used.
 template <int DT>
 __global__ __launch_bounds__(kChunkThreads) void chunk_kernel(SampleArgs a) {
   constexpr int kE = Row<DT>::kE;
   constexpr int kSteps = kChunkElements / kChunkThreads / kE;
   constexpr int kPieceSlots = kPieceElements / kE;  // 32 or 64: half a wave's slots, or a wave's
-  __shared__ float s_max[kChunkThreads / 64];
-  __shared__ uint64_t s_sum[kChunkThreads / 64];
-  const int64_t r = blockIdx.x / a.chunks;
-  const int32_t c = (int32_t)(blockIdx.x - r * a.chunks);
+  __shared__ float s_max[2][kChunkThreads / 64];
+  __shared__ uint64_t s_sum[2][kChunkThreads / 64];
+  const int64_t r = blockIdx.x / a.runs;
+  const int32_t run = (int32_t)(blockIdx.x - r * a.runs);
   const int lane = threadIdx.x & 63;
   const int wave = threadIdx.x >> 6;
   const Row<DT> row(a, r);
-  const int32_t slot0 = c * (kSteps * kChunkThreads) + (int32_t)threadIdx.x;
-  float v[kSteps][kE];
+  const int32_t c0 = run * a.run_chunks;
+  const int32_t c1 = c0 + a.run_chunks < a.chunks ? c0 + a.run_chunks : a.chunks;
+  int32_t slot0 = c0 * (kSteps * kChunkThreads) + (int32_t)threadIdx.x;
+  u32x4 raw[kSteps];
 #pragma unroll
-  for (int j = 0; j < kSteps; ++j) row.load(slot0 + j * kChunkThreads, v[j]);
+  for (int j = 0; j < kSteps; ++j) raw[j] = row.request(slot0 + j * kChunkThreads);
   const Params q = row_params(a, r);
-  float top = -INFINITY;
-#pragma unroll
-  for (int j = 0; j < kSteps; ++j) {
-    float m = v[j][0];
-#pragma unroll
-    for (int e = 1; e < kE; ++e) m = fmaxf(m, v[j][e]);
-#pragma unroll
-    for (int d = kPieceSlots / 2; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
-    if (lane % kPieceSlots == 0)
-      a.piece_max[r * a.pieces + (slot0 + j * kChunkThreads) / kPieceSlots] = m;
-    top = fmaxf(top, m);
-  }
-  top = wave_max(top);
-  if (lane == 0) s_max[wave] = top;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kChunkThreads / 64; ++w) top = fmaxf(top, s_max[w]);
-  if (threadIdx.x == 0) a.chunk_max[r * a.chunks + c] = top;
-  if (a.parts > 0 && needs_bins(a, q)) {
-    for (int32_t b = c * kChunkThreads + (int32_t)threadIdx.x; b < kBins; b += a.chunks * kChunkThreads) {
+  if (needs_bins(a, q)) {
+    for (int32_t b = run * kChunkThreads + (int32_t)threadIdx.x; b < kBins; b += a.runs * kChunkThreads) {
       a.bin_mass[r * kBins + b] = 0;
-      a.bin_count[r * kBins + b] = 0;
     }
+    if (run == 0 && threadIdx.x == 0) a.list_count[r] = 0;
   }
-  if (q.greedy || q.k > 0 || q.p < 1.0 || q.m > 0.0) return;
-  uint64_t sum = 0;
-  if (top > -INFINITY) {
-    const Weights w{0x1.71547652b82fep+0 / (double)q.t, (double)top, top, a.frac};
+  // Rows whose whole mass is needed: without a filter, and with a nucleus cut alone.
+  const bool summed = !q.greedy && q.k == 0 && (q.p < 1.0 ? a.parts > 0 : !(q.m > 0.0));
+  for (int32_t c = c0; c < c1; ++c) {
+    const int buf = c & 1;
+    float v[kSteps][kE];
+    if (c > 0 && (c + 1) * (kSteps * kChunkThreads) <= row.vectors) {
 #pragma unroll
-    for (int j = 0; j < kSteps; ++j)
+      for (int j = 0; j < kSteps; ++j)
+        row.template values<true>(slot0 + j * kChunkThreads, raw[j], v[j]);
+    } else {
 #pragma unroll
-      for (int e = 0; e < kE; ++e) sum += w(v[j][e]);
-  }
-  sum = wave_sum(sum);
-  if (lane == 0) s_sum[wave] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) {
+      for (int j = 0; j < kSteps; ++j)
+        row.template values<false>(slot0 + j * kChunkThreads, raw[j], v[j]);
+    }
 #pragma unroll
-    for (int w = 1; w < kChunkThreads / 64; ++w) sum += s_sum[w];
-    a.chunk_mass[r * a.chunks + c] = sum;
+    for (int j = 0; j < kSteps; ++j)  // (behind the last chunk: the last vector again)
+      raw[j] = row.request(c + 1 < c1 ? slot0 + (kSteps + j) * kChunkThreads : 0);
+    float top = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) {
+      float m = v[j][0];
+#pragma unroll
+      for (int e = 1; e < kE; ++e) m = fmaxf(m, v[j][e]);
+      m = max_to_31(m);
+      if (kPieceSlots == 64) m = max_to_63(m);
+      if (lane % kPieceSlots == kPieceSlots - 1)
+        a.piece_max[r * a.pieces + (slot0 + j * kChunkThreads) / kPieceSlots] = m;
+      top = fmaxf(top, m);
+    }
+    if (kPieceSlots == 32) top = max_to_63(top);
+    if (lane == 63) s_max[buf][wave] = top;
+    lds_barrier();
+    top = s_max[buf][0];
+#pragma unroll
+    for (int w = 1; w < kChunkThreads / 64; ++w) top = fmaxf(top, s_max[buf][w]);
+    if (threadIdx.x == 0) a.chunk_max[r * a.chunks + c] = top;
+    if (summed) {
+      uint64_t sum = 0;
+      if (FastWeights::fits(q.t, top)) {
+        const FastWeights w(q.t, top, a.frac);
+        double part = 0x1p52;
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j)
+#pragma unroll
+          for (int e = 0; e < kE; ++e) part = w.add(v[j][e], part);
+        sum = FastWeights::value(part);
+      } else if (top > -INFINITY) {
+        const Weights w{0x1.71547652b82fep+0 / (double)q.t, (double)top, top, a.frac};
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j)
+#pragma unroll
+          for (int e = 0; e < kE; ++e) sum += w(v[j][e]);
+      }
+      sum = wave_sum(sum);
+      if (lane == 0) s_sum[buf][wave] = sum;
+      lds_barrier();
+      if (threadIdx.x == 0) {
+#pragma unroll
+        for (int w = 1; w < kChunkThreads / 64; ++w) sum += s_sum[buf][w];
+        a.chunk_mass[r * a.chunks + c] = sum;
+      }
+    }
+    slot0 += kSteps * kChunkThreads;
   }
 }
 
@@ -354,35 +466,179 @@ __device__ __forceinline__ float row_max(const SampleArgs& a, int64_t r, float* 
   return m;
 }
 
+// The row's mass from its chunks', each scaled from its own maximum to the row's (one chunk per
+// thread): returns the mass before this thread's chunk; `factor` is its scale.
+__device__ __forceinline__ uint64_t scan_chunks(const SampleArgs& a, int64_t r, const Params& q,
+                                                float top, uint64_t* s_wave, float& chunk_top,
+                                                uint64_t& own, uint64_t& mass, double& factor,
+                                                uint64_t& total) {
+  const int32_t t = threadIdx.x;
+  own = mass = 0;
+  factor = 1.0;
+  chunk_top = -INFINITY;
+  if (t < a.chunks) {
+    chunk_top = a.chunk_max[r * a.chunks + t];
+    mass = own = a.chunk_mass[r * a.chunks + t];
+    if (chunk_top < top) {
+      factor = exp2(fmax(((double)chunk_top - (double)top) * (0x1.71547652b82fep+0 / (double)q.t), -200.0));
+      mass = (uint64_t)rint((double)own * factor);
+    }
+  }
+  return workgroup_scan<uint64_t>(mass, s_wave, total);
+}
+
+// Tiles of a row: 1, 2, 4 ... pieces, at most kMaxTiles of them, each a power of two of slots.
+template <int DT>
+struct Tiles {
+  int32_t count, shift, slots;  // slots = 1 << shift
+  int32_t pieces_shift;
+
+  __device__ __forceinline__ explicit Tiles(const SampleArgs& a) {
+    pieces_shift = 0;
+    while ((a.pieces >> pieces_shift) > kMaxTiles) ++pieces_shift;
+    count = (a.pieces + (1 << pieces_shift) - 1) >> pieces_shift;
+    shift = (Row<DT>::kE == 8 ? 5 : 6) + pieces_shift;
+    slots = 1 << shift;
+  }
+  // The tile of a token.
+  __device__ __forceinline__ int32_t of(const Row<DT>& row, int32_t index) const {
+    constexpr int kShift = Row<DT>::kE == 8 ? 3 : 2;
+    return (index < row.head ? 0 : 1 + ((index - row.head) >> kShift)) >> shift;
+  }
+  __device__ __forceinline__ float max_of(const SampleArgs& a, int64_t r, int32_t tile) const {
+    float m = -INFINITY;
+    for (int32_t i = tile << pieces_shift; i < (tile + 1) << pieces_shift && i < a.pieces; ++i)
+      m = fmaxf(m, a.piece_max[r * a.pieces + i]);
+    return m;
+  }
+};
+
+// Reads the tiles visit[0 .. visits), four slots per thread at a time and the next four in flight,
+// and calls token(value, index) for every token that is at least `from` (not -inf), by whole waves: what a
+// round finds is queued first.  One workgroup; queue.length is 0 before and after.
+template <int DT, typename Token>
+__device__ __forceinline__ void read_tiles(const Row<DT>& row, const Tiles<DT>& tiles,
+                                           const int32_t* visit, int32_t visits, float from,
+                                           Queue& queue, Token token) {
+  constexpr int kE = Row<DT>::kE;
+  constexpr int kTogether = 4;
+  const int lane = threadIdx.x & 63;
+  const int32_t items = visits << tiles.shift;
+  const float least = fmaxf(from, -3.4028235e38f);
+  const auto slot_of = [&](int32_t i) {
+    return i < items ? (visit[i >> tiles.shift] << tiles.shift) + (i & (tiles.slots - 1)) : -1;
+  };
+  u32x4 raw[kTogether];
+#pragma unroll
+  for (int u = 0; u < kTogether; ++u) raw[u] = row.request(slot_of(u * kThreads + (int32_t)threadIdx.x));
+  for (int32_t i0 = 0; i0 < items; i0 += kTogether * kThreads) {
+    float v[kTogether][kE];
+    int32_t slot[kTogether];
+    uint32_t hits = 0;  // one bit per value
+#pragma unroll
+    for (int u = 0; u < kTogether; ++u) {
+      slot[u] = slot_of(i0 + u * kThreads + (int32_t)threadIdx.x);
+      if (slot[u] >= 0) {
+        row.template values<false>(slot[u], raw[u], v[u]);
+#pragma unroll
+        for (int j = 0; j < kE; ++j) hits |= v[u][j] >= least ? 1u << (u * kE + j) : 0u;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kTogether; ++u)
+      raw[u] = row.request(slot_of(i0 + (kTogether + u) * kThreads + (int32_t)threadIdx.x));
+    // (Barriers that leave the requests in flight.)
+    for (int32_t found = kQueue + 1; found > kQueue;) {
+      const uint32_t n = (uint32_t)__popc(hits);
+      const uint32_t incl = wave_scan<uint32_t>(n);
+      const uint32_t all = last_lane(incl);
+      if (all > 0) {  // (uniform)
+        int32_t at = 0;
+        if (lane == 63) at = atomicAdd(&queue.length, (int32_t)all);
+        at = (int32_t)last_lane((uint32_t)at) + (int32_t)(incl - n);
+#pragma unroll
+        for (int u = 0; u < kTogether; ++u)
+#pragma unroll
+          for (int j = 0; j < kE; ++j) {
+            constexpr uint32_t one = 1u;
+            if ((hits & (one << (u * kE + j))) && at < kQueue) {
+              queue.value[at] = v[u][j];
+              queue.index[at] = row.first(slot[u]) + j;
+              ++at;
+              hits &= ~(one << (u * kE + j));
+            }
+          }
+      }
+      lds_barrier();
+      found = queue.length;
+      if (found == 0) break;
+      const int32_t queued = found < kQueue ? found : kQueue;
+      for (int32_t i = threadIdx.x; i < queued; i += kThreads) token(queue.value[i], queue.index[i]);
+      lds_barrier();
+      if (threadIdx.x == 0) queue.length = 0;
+      lds_barrier();
+    }
+  }
+}
+
 // ------------------------------------------------------------------------ histogram pass
-// One part of one row: its tokens and weights per bin, added to the row's (integers: in any order).
+// One part of one row with a nucleus cut alone: the weights of its tokens per bin, added to the
+// row's (integers: in any order).  Tokens with w < (1 - p) Z / vocab cannot be kept (they and all
+// behind them weigh less than (1 - p) Z together) and are left out.  Two copies of the histogram
+// lie interleaved, a lane's copy by its number: most tokens fall into about a hundred bins, and
+// lanes that meet on one address go one after the other.
+struct PartShared {
+  Queue queue;
+  uint64_t mass[2 * kBins];
+  int32_t visit[kMaxTiles];
+  uint64_t wave64[kWaves];
+  float wave_max[kWaves];
+  int32_t visits;
+};
+
+// The least logit that a token of a nucleus can have, with a margin for the roundings.
+__device__ __forceinline__ float nucleus_from(const SampleArgs& a, const Params& q, float top,
+                                              uint64_t total) {
+  if (top == INFINITY) return top;
+  const double z = (double)total * __longlong_as_double((int64_t)(1023 - a.frac) << 52);
+  const double d = -log((1.0 - q.p) * z / (double)a.vocab) * (double)q.t * (1.0 + 0x1p-20);
+  return d > 0.0 ? (float)((double)top - d) - fabsf(top) * 0x1p-20f : top;
+}
+
 template <int DT>
 __global__ __launch_bounds__(kThreads) void bins_kernel(SampleArgs a) {
-  __shared__ uint64_t s_mass[kBins];
-  __shared__ uint32_t s_count[kBins];
-  __shared__ float s_max[kWaves];
+  __shared__ PartShared s;
   const int64_t r = blockIdx.x / a.parts;
   const int32_t part = (int32_t)(blockIdx.x - r * a.parts);
+  const int t = threadIdx.x;
   const Params q = row_params(a, r);
   if (!needs_bins(a, q)) return;
-  const float top = row_max(a, r, s_max);
+  const Tiles<DT> tiles(a);
+  const int32_t per = (tiles.count + a.parts - 1) / a.parts;
+  const int32_t tile = part * per + t;
+  const float tile_max = t < per && tile < tiles.count ? tiles.max_of(a, r, tile) : -INFINITY;
+  for (int32_t b = t; b < 2 * kBins; b += kThreads) s.mass[b] = 0;
+  if (t == 0) s.visits = s.queue.length = 0;
+  const float top = row_max(a, r, s.wave_max);
   if (top == -INFINITY) return;
-  for (int32_t b = threadIdx.x; b < kBins; b += kThreads) {
-    s_mass[b] = 0;
-    s_count[b] = 0;
-  }
+  float chunk_top;
+  uint64_t own, mass, total;
+  double factor;
+  scan_chunks(a, r, q, top, s.wave64, chunk_top, own, mass, factor, total);
+  const float from = nucleus_from(a, q, top, total);
+  if (tile_max >= from && tile_max > -INFINITY) s.visit[atomicAdd(&s.visits, 1)] = tile;
   __syncthreads();
   const Row<DT> row(a, r);
   const Weights w{0x1.71547652b82fep+0 / (double)q.t, (double)top, top, a.frac};
-  const int32_t per = (row.slots() + a.parts - 1) / a.parts;
-  const int32_t s1 = (part + 1) * per < row.slots() ? (part + 1) * per : row.slots();
-  add_to_bins(row, w, q, part * per, s1, s_mass, s_count);
+  read_tiles(row, tiles, s.visit, s.visits, from, s.queue, [&](float v, int32_t) {
+    atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[2 * bin_of(v, top) + (t & 1)]),
+              (unsigned long long)w(v));
+  });
   __syncthreads();
-  for (int32_t b = threadIdx.x; b < kBins; b += kThreads) {
-    if (s_mass[b])
-      atomicAdd(reinterpret_cast<unsigned long long*>(&a.bin_mass[r * kBins + b]),
-                (unsigned long long)s_mass[b]);
-    if (s_count[b]) atomicAdd(&a.bin_count[r * kBins + b], s_count[b]);
+  for (int32_t b = t; b < kBins; b += kThreads) {
+    const uint64_t m = s.mass[2 * b] + s.mass[2 * b + 1];
+    if (m)
+      atomicAdd(reinterpret_cast<unsigned long long*>(&a.bin_mass[r * kBins + b]), (unsigned long long)m);
   }
 }
 
@@ -534,14 +790,16 @@ struct RowShared {
       uint32_t bin_count[kBins];
     } list;
   };
+  Queue queue;
   uint64_t tile_mass[kMaxTiles];
-  float tile_max[kMaxTiles];
   uint32_t tile_ties[kMaxTiles];
+  int32_t visit[kMaxTiles];
   uint64_t wave64[kWaves];
   uint32_t wave32[kWaves];
   float wave_max[kWaves];
   uint64_t value64[4];
   int32_t value32[8];
+  int32_t visits, length;
 };
 
 // Sorts N = kThreads * P places, largest first: value e of thread t is number t P + e.  Partners
@@ -591,27 +849,50 @@ __device__ __forceinline__ void sort_places(uint64_t (&x)[P], uint64_t* s) {
   }
 }
 
-// What the exact order of the list means for the row (cut_list): everything before the list
-// (base tokens and mass per group) and where its two groups lie.
+// The order of at most kRanked places: four threads per place count the larger ones.
+constexpr int kRanked = kThreads / 4;
+__device__ __forceinline__ uint64_t rank_places(int32_t n, uint64_t* s) {
+  uint64_t* sorted = s + kRanked;
+  int32_t* rank = reinterpret_cast<int32_t*>(s + 2 * kRanked);
+  const int t = threadIdx.x;
+  const int e = t % kRanked;
+  if (t < kRanked) rank[t] = 0;
+  __syncthreads();
+  const int32_t per = (n + 3) / 4;
+  const int32_t j0 = t / kRanked * per;
+  const int32_t j1 = j0 + per < n ? j0 + per : n;
+  if (e < n) {
+    const uint64_t mine = s[e];
+    int32_t above = 0;
+    for (int32_t j = j0; j < j1; ++j) above += s[j] > mine ? 1 : 0;
+    if (above) atomicAdd(&rank[e], above);
+  }
+  __syncthreads();
+  if (t < n) sorted[rank[t]] = s[t];  // (n <= kRanked; places differ)
+  __syncthreads();
+  return t < n ? sorted[t] : 0;
+}
+
+// What comes before the list of a row: the mass of the tokens before it, and, with top-p alone, the
+// whole row's (else the list holds all tokens that count).
 struct ListCut {
-  bool top_k, top_p;
-  uint32_t k_left;     // tokens that top-k still keeps of its group
-  int32_t k_group;     // list position where top-k's group begins
-  uint64_t k_mass;     // mass before top-k's group
-  uint64_t p_mass;     // mass before the list's first token
-  uint64_t all_mass;   // the whole row's (top-p without top-k) ...
-  bool whole;          // ... or the list's, if it holds every live token
+  uint64_t before;
+  uint64_t all_mass;
 };
 
 // Sorts the list's n places and finds the last kept one.
 template <int P>
-__device__ uint64_t cut_list(const Weights& w, const Params& q, const ListCut& cut, int32_t n,
+__device__ __forceinline__ uint64_t cut_list(const Weights& w, const Params& q, const ListCut& cut, int32_t n,
                              RowShared& s) {
   uint64_t x[P];
   const int t = threadIdx.x;
+  if constexpr (P == 1) {
+    x[0] = rank_places(n, s.list.place);  // (at most kRanked)
+  } else {
 #pragma unroll
-  for (int e = 0; e < P; ++e) x[e] = t * P + e < n ? s.list.place[t * P + e] : 0;
-  sort_places<P>(x, s.list.place);
+    for (int e = 0; e < P; ++e) x[e] = t * P + e < n ? s.list.place[t * P + e] : 0;
+    sort_places<P>(x, s.list.place);
+  }
   uint64_t weight[P];
   uint64_t sum = 0;
 #pragma unroll
@@ -622,32 +903,27 @@ __device__ uint64_t cut_list(const Weights& w, const Params& q, const ListCut& c
   __syncthreads();
   uint64_t total;
   const uint64_t before = workgroup_scan<uint64_t>(sum, s.wave64, total);
-  // S(n_k): the mass before top-k's group and of the tokens it keeps of it.  Position of the last.
-  const int32_t k_last = cut.top_k ? cut.k_group + (int32_t)cut.k_left - 1 : n - 1;
+  // S(n_k): of the first k, or everything.
+  const bool top_k = q.k > 0 && q.k < n;
+  int32_t last = top_k ? q.k - 1 : n - 1;
   if (t == 0) {
-    s.value64[0] = 0;
-    s.value64[1] = 0;
     s.value32[0] = -1;
+    s.value64[2] = 0;
   }
   __syncthreads();
-  uint64_t at = before;
+  if (q.p < 1.0) {
+    uint64_t at = before;
 #pragma unroll
-  for (int e = 0; e < P; ++e) {
-    const int32_t i = t * P + e;
-    if (i == cut.k_group) s.value64[0] = at;
-    at += weight[e];
-    if (i == k_last) s.value64[1] = at;
-  }
-  __syncthreads();
-  int32_t last = k_last;
-  if (cut.top_p) {
-    const uint64_t kept = cut.top_k   ? cut.k_mass + (s.value64[1] - s.value64[0])
-                          : cut.whole ? total
-                                      : cut.all_mass;
+    for (int e = 0; e < P; ++e) {
+      at += weight[e];
+      if (t * P + e == last) s.value64[0] = at;
+    }
+    __syncthreads();
+    const uint64_t kept = q.k > 0 || cut.all_mass == 0 ? s.value64[0] : cut.all_mass;
     // Tokens whose preceding mass is below p S(n_k).
     uint64_t want = (uint64_t)ceil(q.p * (double)kept);
     want = want < 1 ? 1 : want;
-    at = cut.p_mass + before;
+    at = cut.before + before;
     int32_t mine = -1;
 #pragma unroll
     for (int e = 0; e < P; ++e) {
@@ -669,40 +945,133 @@ __device__ uint64_t cut_list(const Weights& w, const Params& q, const ListCut& c
   return s.value64[2];
 }
 
+// The members of one sub-bin of the list, in order: thread i gets the i-th of `count` (more than
+// kRanked: they are not ordered).  They are put behind the list's n places.
+template <typename SubBin>
+__device__ __forceinline__ uint64_t members(int32_t n, int32_t bin, SubBin sub_bin, RowShared& s,
+                                            int32_t& count) {
+  uint64_t* found = reinterpret_cast<uint64_t*>(&s.queue);
+  if (threadIdx.x == 0) s.length = 0;
+  __syncthreads();
+  for (int32_t i = threadIdx.x; i < n; i += kThreads)
+    if (sub_bin(s.list.place[i]) == bin) {
+      const int32_t at = atomicAdd(&s.length, 1);
+      if (at < kRanked) found[at] = s.list.place[i];
+    }
+  __syncthreads();
+  count = s.length;
+  return count <= kRanked ? rank_places(count, found) : 0;
+}
+
+// The last kept place of a longer list: its tokens' counts and masses in sub-bins of equal key
+// ranges, then the exact order within the two sub-bins where the cuts fall.  False if one of those
+// holds too many (equal logits).
+__device__ __forceinline__ bool cut_by_bins(const Weights& w, const Params& q, const ListCut& cut,
+                                            int32_t n, RowShared& s, uint64_t& last) {
+  constexpr int kSub = 2 * kThreads;
+  static_assert(kSub <= kBins, "the row's bins are reused");
+  const int t = threadIdx.x;
+  uint32_t high = 0, low = 0xffffffffu;
+  for (int32_t i = t; i < n; i += kThreads) {
+    const uint32_t k = place_key(s.list.place[i]);
+    high = k > high ? k : high;
+    low = k < low ? k : low;
+  }
+  if (t == 0) {
+    s.wave32[0] = 0;
+    s.wave32[1] = 0xffffffffu;
+  }
+  for (int32_t b = t; b < kSub; b += kThreads) {
+    s.list.bin_mass[b] = 0;
+    s.list.bin_count[b] = 0;
+  }
+  __syncthreads();
+  high = wave_extreme<true>(high);
+  low = wave_extreme<false>(low);
+  if ((t & 63) == 63) {
+    atomicMax(&s.wave32[0], high);
+    atomicMin(&s.wave32[1], low);
+  }
+  __syncthreads();
+  high = s.wave32[0];
+  const uint32_t range = high - s.wave32[1];
+  const int shift = range < (uint32_t)kSub ? 0 : 32 - 11 - __clz((int)range);  // range >> shift < kSub
+  const auto sub_bin = [&](uint64_t place) { return (int32_t)((high - place_key(place)) >> shift); };
+  for (int32_t i = t; i < n; i += kThreads) {
+    const uint64_t p = s.list.place[i];
+    const int32_t b = sub_bin(p);
+    atomicAdd(&s.list.bin_count[b], 1u);
+    if (q.p < 1.0)
+      atomicAdd(reinterpret_cast<unsigned long long*>(&s.list.bin_mass[b]),
+                (unsigned long long)w(value_of(place_key(p))));
+  }
+  __syncthreads();
+  const uint32_t c0 = s.list.bin_count[2 * t], c1 = s.list.bin_count[2 * t + 1];
+  const uint64_t m0 = s.list.bin_mass[2 * t], m1 = s.list.bin_mass[2 * t + 1];
+  uint32_t count_all;
+  uint64_t mass_all = 0, mb = 0;
+  const uint32_t cb = workgroup_scan<uint32_t>(c0 + c1, s.wave32, count_all);
+  if (q.p < 1.0) mb = workgroup_scan<uint64_t>(m0 + m1, s.wave64, mass_all);
+  const bool top_k = q.k > 0 && q.k < n;
+  uint64_t kept = mass_all;
+  last = 0;  // (everything)
+  int32_t count;
+  if (top_k) {
+    const uint32_t k = (uint32_t)q.k;
+    if (cb < k && k <= cb + c0 + c1) {  // one thread
+      const bool second = cb + c0 < k;
+      s.value32[6] = second ? 2 * t + 1 : 2 * t;
+      s.value32[7] = (int32_t)(k - (second ? cb + c0 : cb));
+      s.value64[0] = second ? mb + m0 : mb;
+    }
+    __syncthreads();
+    const int32_t left = s.value32[7];
+    kept = s.value64[0];
+    const uint64_t place = members(n, s.value32[6], sub_bin, s, count);
+    if (count > kRanked) return false;
+    if (t == left - 1) s.value64[1] = place;
+    uint64_t sum = 0;
+    if (q.p < 1.0)
+      workgroup_scan<uint64_t>(t < left ? w(value_of(place_key(place))) : 0, s.wave64, sum);
+    else
+      __syncthreads();
+    kept += sum;
+    last = s.value64[1];
+    __syncthreads();
+  } else if (q.k == 0 && cut.all_mass > 0) {
+    kept = cut.all_mass;
+  }
+  if (q.p < 1.0) {
+    uint64_t want = (uint64_t)ceil(q.p * (double)kept);
+    want = want < 1 ? 1 : want;
+    want = want > cut.before ? want - cut.before : 1;
+    want = want < mass_all ? want : mass_all;
+    if (mb < want && want <= mb + m0 + m1) {  // one thread
+      const bool second = mb + m0 < want;
+      s.value32[6] = second ? 2 * t + 1 : 2 * t;
+      s.value64[0] = second ? mb + m0 : mb;
+    }
+    __syncthreads();
+    const uint64_t before_bin = s.value64[0];
+    const uint64_t place = members(n, s.value32[6], sub_bin, s, count);
+    if (count > kRanked) return false;
+    const uint64_t mass = t < count ? w(value_of(place_key(place))) : 0;
+    uint64_t sum;
+    const uint64_t at = before_bin + workgroup_scan<uint64_t>(mass, s.wave64, sum);
+    if (at < want && want <= at + mass) s.value64[1] = place;  // one thread
+    __syncthreads();
+    last = s.value64[1];
+    __syncthreads();
+  }
+  return true;
+}
+
 __device__ __forceinline__ uint64_t cut_list_any(const Weights& w, const Params& q,
                                                  const ListCut& cut, int32_t n, RowShared& s) {
-  if (n <= kThreads) return cut_list<1>(w, q, cut, n, s);
-  if (n <= 2 * kThreads) return cut_list<2>(w, q, cut, n, s);
-  return cut_list<4>(w, q, cut, n, s);
-}
-
-// Adds this lane's tokens to the list (those with `in`); more than kList of them only count.
-__device__ __forceinline__ void append(bool in, uint64_t place, RowShared& s) {
-  const uint64_t mask = __ballot(in);
-  if (mask == 0) return;
-  const int lane = threadIdx.x & 63;
-  const int leader = __ffsll((unsigned long long)mask) - 1;
-  int32_t at = 0;
-  if (lane == leader) at = atomicAdd(&s.value32[1], (int32_t)__popcll(mask));
-  at = __shfl(at, leader, 64) + (int32_t)__popcll(mask & (((uint64_t)1 << lane) - 1));
-  if (in && at < kList) s.list.place[at] = place;
-}
-
-// The k-th largest of the tiles' maxima (k <= tiles).
-__device__ float kth_tile_max(const SampleArgs& a, int32_t k, int32_t tiles, RowShared& s) {
-  uint64_t x[1];
-  x[0] = (int32_t)threadIdx.x < tiles ? place_of(key_of(s.tile_max[threadIdx.x]), threadIdx.x) : 0;
-  sort_places<1>(x, s.list.place);
-  if ((int32_t)threadIdx.x == k - 1) s.value64[3] = x[0];
-  __syncthreads();
-  const float v = value_of(place_key(s.value64[3]));
-  __syncthreads();
-  return v;
-}
-
-template <int DT>
-__device__ __forceinline__ int32_t tile_of(const Row<DT>& row, int32_t index, int32_t tile_slots) {
-  return (index < row.head ? 0 : 1 + (index - row.head) / Row<DT>::kE) / tile_slots;
+  if (n <= kRanked) return cut_list<1>(w, q, cut, n, s);
+  uint64_t last;
+  if (cut_by_bins(w, q, cut, n, s, last)) return last;
+  return cut_list<kList / kThreads>(w, q, cut, n, s);
 }
 
 // The first token, in index order, at which the kept weight exceeds `target`, within the slots
@@ -723,7 +1092,7 @@ __device__ __forceinline__ int32_t pick_in_slots(const Row<DT>& row, int32_t s0,
       x[j] = q < s1 ? weight_of(v[j], row.first(q) + j) : 0;
       mass += x[j];
     }
-    const uint64_t incl = wave_scan<unsigned long long>(mass);
+    const uint64_t incl = wave_scan<uint64_t>(mass);
     const uint64_t before = incl - mass;
     const bool here = before <= target && target < incl;
     const uint64_t any = __ballot(here);
@@ -748,29 +1117,20 @@ __device__ __forceinline__ int32_t pick_in_slots(const Row<DT>& row, int32_t s0,
 
 // Rows without a filter: the chunk that holds the target from the chunks' masses, then the token.
 template <int DT>
-__device__ void finish_plain(const SampleArgs& a, const Row<DT>& row, int64_t r, const Params& q,
+__device__ __forceinline__ void finish_plain(const SampleArgs& a, const Row<DT>& row, int64_t r, const Params& q,
                              float top, RowShared& s) {
-  constexpr int kChunkSlots = kChunkElements / Row<DT>::kE;
+  constexpr int kE = Row<DT>::kE;
+  constexpr int kChunkSlots = kChunkElements / kE;  // at most kThreads
   const int t = threadIdx.x;
   const double c = 0x1.71547652b82fep+0 / (double)q.t;
-  uint64_t mass = 0, own = 0;
-  double factor = 1.0;
-  float m = -INFINITY;
-  if (t < a.chunks) {
-    m = a.chunk_max[r * a.chunks + t];
-    own = a.chunk_mass[r * a.chunks + t];
-    mass = own;
-    if (m < top) {
-      factor = exp2(fmax(((double)m - (double)top) * c, -200.0));
-      mass = (uint64_t)rint((double)own * factor);
-    }
-  }
   if (t == 0) {
     s.value64[0] = 0;
     s.value32[0] = 0;
   }
-  uint64_t total;
-  const uint64_t before = workgroup_scan<uint64_t>(mass, s.wave64, total);
+  float m;
+  uint64_t own, mass, total;
+  double factor;
+  const uint64_t before = scan_chunks(a, r, q, top, s.wave64, m, own, mass, factor, total);
   const uint64_t target = scaled(q.u, total);
   if (before <= target && target < before + mass) {  // one thread
     uint64_t left = target - before;
@@ -780,14 +1140,40 @@ __device__ void finish_plain(const SampleArgs& a, const Row<DT>& row, int64_t r,
     s.wave_max[0] = m;
   }
   __syncthreads();
-  if (t < 64) {
-    const float cm = s.wave_max[0];
+  // The chunk's slots, one per thread.
+  const float cm = s.wave_max[0];
+  uint64_t left = s.value64[0];
+  const int32_t slot = s.value32[0] * kChunkSlots + t;
+  float v[kE];
+  uint64_t x[kE];
+  uint64_t sum = 0;
+  row.load(t < kChunkSlots ? slot : row.slots(), v);  // (past the row: -inf)
+  if (FastWeights::fits(q.t, cm)) {
+    const FastWeights w(q.t, cm, a.frac);
+#pragma unroll
+    for (int j = 0; j < kE; ++j) x[j] = w(v[j]);
+  } else {
     const Weights w{c, (double)cm, cm, a.frac};
-    const int32_t s0 = s.value32[0] * kChunkSlots;
-    const int32_t s1 = s0 + kChunkSlots < row.slots() ? s0 + kChunkSlots : row.slots();
-    const int32_t pick =
-        pick_in_slots(row, s0, s1, s.value64[0], [&](float v, int32_t) { return w(v); });
-    if (t == 0) a.out[r] = pick;
+#pragma unroll
+    for (int j = 0; j < kE; ++j) x[j] = w(v[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < kE; ++j) sum += x[j];
+  uint64_t all;
+  uint64_t at = workgroup_scan<uint64_t>(sum, s.wave64, all);
+  if (left >= all) left = all - 1;  // (a sum of several weights may round otherwise than each)
+  if (at <= left && left < at + sum) {  // one thread
+    int32_t pick = 0;
+    bool done = false;
+#pragma unroll
+    for (int j = 0; j < kE; ++j) {
+      at += x[j];
+      if (!done && at > left) {
+        pick = row.first(slot) + j;
+        done = true;
+      }
+    }
+    a.out[r] = pick;
   }
 }
 
@@ -819,10 +1205,15 @@ __device__ __forceinline__ void finish_tiles(const SampleArgs& a, const Row<DT>&
 }
 
 // The general path: cut by digits, then the kept weight of every tile, ties counted by index.
+// (Not inlined, and given a copy of the arguments: the row kernel keeps its registers.)
 template <int DT>
-__device__ void finish_general(const SampleArgs& a, const Row<DT>& row, int64_t r, const Weights& w,
-                               const Params& q, uint64_t least, int32_t tiles, int32_t tile_slots,
-                               RowShared& s) {
+__device__ __attribute__((noinline)) void finish_general(const SampleArgs& a, int64_t r, float top,
+                                                         RowShared& s) {
+  const Row<DT> row(a, r);
+  const Params q = row_params(a, r);
+  const Weights w{0x1.71547652b82fep+0 / (double)q.t, (double)top, top, a.frac};
+  const uint64_t least = least_weight(q.m, a.frac);
+  const int32_t tiles = Tiles<DT>(a).count, tile_slots = Tiles<DT>(a).slots;
   const int lane = threadIdx.x & 63;
   const int wave = threadIdx.x >> 6;
   __syncthreads();
@@ -887,202 +1278,251 @@ __device__ void finish_general(const SampleArgs& a, const Row<DT>& row, int64_t 
   });
 }
 
+// The bin in which the cumulative sum of s.list.bin_mass (or bin_count) reaches `want`, and what
+// comes before that bin; kBins if the whole does not reach it.
+template <typename T>
+__device__ __forceinline__ int32_t find_bin(const T* bins, T want, T* s_wave, RowShared& s, T& before,
+                                            T& total) {
+  const int32_t b0 = (int32_t)threadIdx.x * kThreadBins;
+  T x[kThreadBins];
+  T sum = 0;
+#pragma unroll
+  for (int j = 0; j < kThreadBins; ++j) {
+    x[j] = b0 + j < kBins ? bins[b0 + j] : 0;
+    sum += x[j];
+  }
+  if (threadIdx.x == 0) s.value32[6] = kBins;
+  T at = workgroup_scan<T>(sum, s_wave, total);
+  if (at < want && want <= at + sum) {  // one thread
+    int32_t bin = b0;
+#pragma unroll
+    for (int j = 0; j < kThreadBins; ++j)
+      if (at < want && want <= at + x[j]) {
+        bin = b0 + j;
+        s.value64[0] = at;
+        at = want;  // (found)
+      } else {
+        at += x[j];
+      }
+    s.value32[6] = bin;
+  }
+  __syncthreads();
+  before = (T)s.value64[0];
+  const int32_t bin = s.value32[6];
+  __syncthreads();
+  return bin;
+}
+
+// The bin in which a nucleus cut alone falls (histogram in s.list.bin_mass, `total` the row's mass).
+__device__ __forceinline__ int32_t nucleus_bin(const Params& q, uint64_t total, RowShared& s,
+                                               uint64_t& before, uint64_t& binned) {
+  const uint64_t want = (uint64_t)ceil(q.p * (double)total);
+  int32_t bin = find_bin<uint64_t>(s.list.bin_mass, want < 1 ? 1 : want, s.wave64, s, before, binned);
+  // (Roundings: the tokens left out weigh less than (1 - p) Z, but p Z may be all but Z.)
+  if (bin == kBins) bin = find_bin<uint64_t>(s.list.bin_mass, binned, s.wave64, s, before, binned);
+  return bin;
+}
+
+// The smallest value of a bin, or a little less.
+__device__ __forceinline__ float bin_from(int32_t bin, float top) {
+  if (bin >= kBins - 1) return -INFINITY;
+  if (top == INFINITY) return top;
+  const float d = __uint_as_float((uint32_t)(bin + kBinBase) << kBinShift);  // the next bin's least d
+  return (float)((double)top - (double)d) - fabsf(top) * 0x1p-20f;
+}
+
+// Puts the tokens down to bin `last` where they belong: those of bins from `first` on into
+// s.list.place, the weights of those before it to s.tile_mass (tile `base` first), `least` and
+// more.  s.visit, s.visits, s.length and s.queue.length are set.
+template <int DT>
+__device__ __forceinline__ void gather(const Row<DT>& row, const Tiles<DT>& tiles, const Weights& w,
+                                       int32_t first, int32_t last, uint64_t least, int32_t base,
+                                       RowShared& s) {
+  const float top = w.topf;
+  read_tiles(row, tiles, s.visit, s.visits, bin_from(last, top), s.queue, [&](float v, int32_t index) {
+    const int32_t b = bin_of(v, top);
+    if (b < first) {
+      const uint64_t x = w(v);
+      if (x >= least && x > 0)
+        atomicAdd(reinterpret_cast<unsigned long long*>(&s.tile_mass[tiles.of(row, index) - base]),
+                  (unsigned long long)x);
+    } else if (b <= last) {
+      const int32_t at = atomicAdd(&s.length, 1);
+      if (at < kList) s.list.place[at] = place_of(key_of(v), index);
+    }
+  });
+}
+
+// One part of the tiles of a row with a nucleus cut alone, its histogram finished: the tokens of
+// the bin where the cut falls, and the mass of those before it per tile.
+template <int DT>
+__global__ __launch_bounds__(kThreads) void gather_kernel(SampleArgs a) {
+  __shared__ RowShared s;
+  const int64_t r = blockIdx.x / a.parts;
+  const int32_t part = (int32_t)(blockIdx.x - r * a.parts);
+  const int t = threadIdx.x;
+  const Params q = row_params(a, r);
+  if (!needs_bins(a, q)) return;
+  const Tiles<DT> tiles(a);
+  const int32_t per = (tiles.count + a.parts - 1) / a.parts;
+  const int32_t tile0 = part * per;
+  const int32_t tile1 = tile0 + per < tiles.count ? tile0 + per : tiles.count;
+  if (tile0 >= tile1) return;
+  for (int32_t b = t; b < kBins; b += kThreads) s.list.bin_mass[b] = a.bin_mass[r * kBins + b];
+  const float tile_max = t < tile1 - tile0 ? tiles.max_of(a, r, tile0 + t) : -INFINITY;
+  if (t == 0) s.visits = s.length = s.queue.length = 0;
+  s.tile_mass[t] = 0;
+  const float top = row_max(a, r, s.wave_max);  // (with a barrier)
+  if (top == -INFINITY) return;
+  const Row<DT> row(a, r);
+  const Weights w{0x1.71547652b82fep+0 / (double)q.t, (double)top, top, a.frac};
+  float chunk_top;
+  uint64_t own, mass, total, before, binned;
+  double factor;
+  scan_chunks(a, r, q, top, s.wave64, chunk_top, own, mass, factor, total);
+  const int32_t bin = nucleus_bin(q, total, s, before, binned);
+  if (tile_max >= bin_from(bin, top) && tile_max > -INFINITY)
+    s.visit[atomicAdd(&s.visits, 1)] = tile0 + t;
+  __syncthreads();
+  gather(row, tiles, w, bin, bin, least_weight(q.m, a.frac), tile0, s);
+  __syncthreads();
+  if (t < tile1 - tile0) a.tile_mass[r * kMaxTiles + tile0 + t] = s.tile_mass[t];
+  const int32_t n = s.length;
+  if (t == 0) s.value32[6] = n > 0 ? atomicAdd(&a.list_count[r], n) : 0;
+  __syncthreads();
+  const int32_t at = s.value32[6];
+  for (int32_t i = t; i < n && i < kList && at + i < kList; i += kThreads)
+    a.list[r * kList + at + i] = s.list.place[i];
+}
+
 // One row.  Rows without a filter need the chunks' masses only.  Otherwise the cut lies in a list
-// of tokens that are put in exact order: with a top-k of at most half the pieces, all tokens at or
-// above the k-th largest piece maximum (at least k of them, hardly more than twice k); else the
-// tokens of the bins that the cuts fall into.  Tiles whose maximum shows that they hold no kept
-// token are not read.
+// of tokens that are put in exact order: with a nucleus cut alone those that gather_kernel left,
+// else all tokens down to a logit that the piece maxima give.  For a top-k of at most half the
+// pieces that is the k-th largest of them (at least k tokens, hardly more than twice as many); for
+// a larger one a guess, as if the pieces were random samples of the row, which the list's length
+// then confirms or not.  Tiles whose maximum shows that they hold no token of the list or before
+// it are not read.
 template <int DT>
 __global__ __launch_bounds__(kThreads) void row_kernel(SampleArgs a) {
-  constexpr int kE = Row<DT>::kE;
   __shared__ RowShared s;
   const int64_t r = blockIdx.x;
   const int t = threadIdx.x;
-  const int lane = t & 63;
-  const int wave = t >> 6;
   const Row<DT> row(a, r);
   const Params q = row_params(a, r);
+  const Tiles<DT> tiles(a);
+  const bool filter = q.k > 0 || q.p < 1.0;
+  const bool counted = needs_bins(a, q);  // histogram and list are there
+  const float tile_max = t < tiles.count ? tiles.max_of(a, r, t) : -INFINITY;
+  s.tile_mass[t] = counted && t < tiles.count ? a.tile_mass[r * kMaxTiles + t] : 0;
+  if (filter)
+    for (int32_t b = t; b < kBins; b += kThreads) {
+      if (counted)
+        s.list.bin_mass[b] = a.bin_mass[r * kBins + b];
+      else
+        s.list.bin_count[b] = 0;
+    }
+  if (t == 0) {
+    s.length = counted ? a.list_count[r] : 0;
+    s.visits = s.queue.length = 0;
+    s.value32[4] = kMaxTiles;  // first tile with the maximum
+  }
   const float top = row_max(a, r, s.wave_max);
   __syncthreads();
   if (top == -INFINITY) {
     if (t == 0) a.out[r] = 0;
     return;
   }
-  const bool filter = q.k > 0 || q.p < 1.0;
-  if (!q.greedy && !filter && !(q.m > 0.0)) {
-    finish_plain(a, row, r, q, top, s);
-    return;
-  }
-  // Tiles: one or more pieces, at most kMaxTiles.
-  const int32_t per_tile = (a.pieces + kMaxTiles - 1) / kMaxTiles;
-  const int32_t tiles = (a.pieces + per_tile - 1) / per_tile;
-  const int32_t tile_slots = per_tile * (kPieceElements / kE);
-  if (t < tiles) {
-    float m = -INFINITY;
-    for (int32_t i = t * per_tile; i < (t + 1) * per_tile && i < a.pieces; ++i)
-      m = fmaxf(m, a.piece_max[r * a.pieces + i]);
-    s.tile_max[t] = m;
-    s.tile_mass[t] = 0;
-  }
-  if (t == 0) {
-    s.value32[1] = 0;           // list length
-    s.value32[4] = kMaxTiles;   // first tile with the maximum
-    s.value32[5] = 0;           // list members before top-k's bin
-  }
-  __syncthreads();
   if (q.greedy) {
-    if (t < tiles && s.tile_max[t] == top) atomicMin(&s.value32[4], t);
+    if (tile_max == top) atomicMin(&s.value32[4], t);
     __syncthreads();
-    if (wave == 0) {
-      const int32_t s0 = s.value32[4] * tile_slots;
-      const int32_t s1 = s0 + tile_slots < row.slots() ? s0 + tile_slots : row.slots();
+    if (t < 64) {
+      const int32_t s0 = s.value32[4] << tiles.shift;
+      const int32_t s1 = s0 + tiles.slots < row.slots() ? s0 + tiles.slots : row.slots();
       const int32_t pick = pick_in_slots(row, s0, s1, 0, [&](float v, int32_t) {
         return (uint64_t)(v == top ? 1 : 0);
       });
-      if (lane == 0) a.out[r] = pick;
+      if (t == 0) a.out[r] = pick;
     }
+    return;
+  }
+  if (!filter && !(q.m > 0.0)) {
+    finish_plain(a, row, r, q, top, s);
     return;
   }
   const Weights w{0x1.71547652b82fep+0 / (double)q.t, (double)top, top, a.frac};
   const uint64_t least = least_weight(q.m, a.frac);
-  ListCut cut{q.k > 0, q.p < 1.0, (uint32_t)q.k, 0, 0, 0, 0, false};
-  int32_t first_bin = kBins, last_bin = -1, k_bin = -1;  // bins of the list: [first, last] and k_bin
-  float list_from = INFINITY;                            // or all tokens from this value on
-  if (filter && by_pieces(a, q) && per_tile == 1) {
-    list_from = kth_tile_max(a, q.k, tiles, s);
-  } else if (filter) {
-    uint64_t* mass = s.list.bin_mass;
-    uint32_t* count = s.list.bin_count;
-    for (int32_t b = t; b < kBins; b += kThreads) {
-      mass[b] = a.parts > 0 && needs_bins(a, q) ? a.bin_mass[r * kBins + b] : 0;
-      count[b] = a.parts > 0 && needs_bins(a, q) ? a.bin_count[r * kBins + b] : 0;
-    }
-    __syncthreads();
-    if (!(a.parts > 0 && needs_bins(a, q))) add_to_bins(row, w, q, 0, row.slots(), mass, count);
-    __syncthreads();
-    // Thread t holds bins 2 t and 2 t + 1: the largest logits first.
-    const int32_t b0 = 2 * t;
-    const bool in0 = b0 < kBins, in1 = b0 + 1 < kBins;
-    const uint64_t m0 = in0 ? mass[b0] : 0, m1 = in1 ? mass[b0 + 1] : 0;
-    const uint32_t c0 = in0 ? count[b0] : 0, c1 = in1 ? count[b0 + 1] : 0;
-    uint64_t all_mass;
-    uint32_t all_count;
-    const uint64_t mb = workgroup_scan<uint64_t>(m0 + m1, s.wave64, all_mass);
-    const uint32_t cb = workgroup_scan<uint32_t>(c0 + c1, s.wave32, all_count);
-    cut.all_mass = all_mass;
-    cut.top_k = q.k > 0 && (uint32_t)q.k < all_count;  // (else it keeps every live token)
-    uint64_t low = all_mass, high = all_mass;           // bounds of S(n_k)
-    if (cut.top_k) {
-      const uint32_t k = (uint32_t)q.k;
-      if (cb < k && k <= cb + c0 + c1) {  // one thread
-        const bool second = cb + c0 < k;
-        s.value32[6] = second ? b0 + 1 : b0;
-        s.value32[7] = (int32_t)(k - (second ? cb + c0 : cb));
-        s.value64[0] = second ? mb + m0 : mb;
-        s.value64[1] = second ? m1 : m0;
-      }
-      __syncthreads();
-      k_bin = s.value32[6];
-      cut.k_left = (uint32_t)s.value32[7];
-      cut.k_mass = low = s.value64[0];
-      high = low + s.value64[1];
-      first_bin = last_bin = k_bin;
-      __syncthreads();
-    }
-    if (cut.top_p) {
-      uint64_t want0 = (uint64_t)ceil(q.p * (double)low), want1 = (uint64_t)ceil(q.p * (double)high);
-      want0 = want0 < 1 ? 1 : want0;
-      want1 = want1 < 1 ? 1 : want1;
-      const uint64_t x1 = mb + m0, x2 = x1 + m1;
-      if (mb < want0 && want0 <= x2) {  // one thread
-        const bool second = x1 < want0;
-        s.value32[6] = second ? b0 + 1 : b0;
-        s.value64[0] = second ? x1 : mb;
-      }
-      if (mb < want1 && want1 <= x2) s.value32[7] = x1 < want1 ? b0 + 1 : b0;
-      __syncthreads();
-      first_bin = s.value32[6];
-      last_bin = s.value32[7];
-      cut.p_mass = s.value64[0];
-      __syncthreads();
-    }
-    if (!cut.top_k && !cut.top_p) first_bin = kBins;  // top-k keeps every live token
-  }
-  // Gather the list; the weights of the tokens before it go to their tiles.
-  const int32_t reach = last_bin > k_bin ? last_bin : k_bin;
-  const bool by_value = list_from < INFINITY;
-  for (int32_t tile = wave; tile < tiles; tile += kWaves) {
-    const float m = s.tile_max[tile];
-    if (m == -INFINITY) continue;
-    if (by_value ? m < list_from : (first_bin < kBins && bin_of(m, top) > reach)) continue;
-    uint64_t mass = 0;
-    for (int32_t i = lane; i < tile_slots; i += 64) {
-      const int32_t slot = tile * tile_slots + i;
-      float v[kE];
-      if (slot < row.slots()) {
-        row.load(slot, v);
-      } else {
-#pragma unroll
-        for (int j = 0; j < kE; ++j) v[j] = -INFINITY;
-      }
-#pragma unroll
-      for (int j = 0; j < kE; ++j) {
-        bool in;
-        if (by_value) {
-          in = v[j] >= list_from && v[j] > -INFINITY;
-        } else {
-          const int32_t b = bin_of(v[j], top);
-          const bool live = v[j] > -INFINITY;
-          in = live && ((b >= first_bin && b <= last_bin) || b == k_bin);
-          if (live && b < first_bin) {
-            const uint64_t x = w(v[j]);
-            mass += x >= least ? x : 0;
-          }
-          const uint64_t before = __ballot(in && b < k_bin);
-          if (before && lane == 0) atomicAdd(&s.value32[5], (int32_t)__popcll(before));
+  ListCut cut{0, 0};
+  bool confirmed = true;
+  if (counted) {
+    float chunk_top;
+    uint64_t own, mass, total, binned;
+    double factor;
+    scan_chunks(a, r, q, top, s.wave64, chunk_top, own, mass, factor, total);
+    nucleus_bin(q, total, s, cut.before, binned);
+    cut.all_mass = total < binned ? binned : total;
+    const int32_t n = s.length < kList ? s.length : kList;
+    for (int32_t i = t; i < n; i += kThreads) s.list.place[i] = a.list[r * kList + i];
+  } else {
+    int32_t last = kBins - 1;
+    if (filter) {
+      if (tile_max > -INFINITY) atomicAdd(&s.list.bin_count[bin_of(tile_max, top)], 1u);
+      const uint32_t live = (uint32_t)__syncthreads_count(tile_max > -INFINITY);
+      // All live tokens fit the list?  Else down to the bin of the `rank`-th largest maximum.
+      if ((live << tiles.pieces_shift) > kList / kPieceElements) {
+        const uint32_t k = (uint32_t)(q.k > 0 ? q.k : a.vocab);
+        uint32_t rank = k, before, all;
+        if (k > live / 2) {
+          const float share = 1.0f - expf(-1.3f * (float)k / (float)live - 0.3f);
+          rank = (uint32_t)ceilf((float)live * share);
+          rank = rank < live ? rank : live;
         }
-        append(in, place_of(key_of(v[j]), row.first(slot) + j), s);
+        last = find_bin<uint32_t>(s.list.bin_count, rank, s.wave32, s, before, all);
+        confirmed = k <= kList;  // (no list could hold it)
       }
+    } else {
+      // min-p alone: w >= m is M - v <= -T ln m (and a little more, for the roundings).
+      const double d = -log(q.m) * (double)q.t * (1.0 + 0x1p-20) + 0x1p-100;
+      last = bin_of((float)((double)top - d) - fabsf(top) * 0x1p-20f, top);
     }
-    if (!by_value) {
-      mass = wave_sum(mass);
-      if (lane == 0) s.tile_mass[tile] = mass;
-    }
+    if (confirmed && tile_max >= bin_from(last, top) && tile_max > -INFINITY)
+      s.visit[atomicAdd(&s.visits, 1)] = t;
+    __syncthreads();
+    // (min-p alone lists nothing: everything goes to the tiles.)
+    gather(row, tiles, w, filter ? 0 : kBins, last, least, 0, s);
+    __syncthreads();
+    // The list holds the first k tokens, or every live one.
+    confirmed = confirmed && (last == kBins - 1 || !filter || s.length >= q.k);
   }
   __syncthreads();
-  const int32_t n = s.value32[1];
-  uint64_t last = 0;
-  if (by_value || first_bin < kBins) {
-    if (n > kList) {
-      finish_general(a, row, r, w, q, least, tiles, tile_slots, s);
+  uint64_t last_place = 0;
+  if (filter) {
+    const int32_t n = s.length;
+    if (n > kList || !confirmed) {
+      const SampleArgs copy = a;
+      finish_general<DT>(copy, r, top, s);
       return;
     }
-    cut.k_group = s.value32[5];
-    if (by_value && n < q.k) {  // fewer live tokens than top-k keeps, and all of them listed
-      cut.top_k = false;
-      cut.whole = true;
-    }
-    last = cut_list_any(w, q, cut, n, s);
+    last_place = cut_list_any(w, q, cut, n, s);
     for (int32_t i = t; i < n; i += kThreads) {
       const uint64_t p = s.list.place[i];
       const uint64_t x = w(value_of(place_key(p)));
-      if (p >= last && x >= least)
+      if (p >= last_place && x >= least)
         atomicAdd(reinterpret_cast<unsigned long long*>(
-                      &s.tile_mass[tile_of(row, place_index(p), tile_slots)]),
+                      &s.tile_mass[tiles.of(row, place_index(p))]),
                   (unsigned long long)x);
     }
     __syncthreads();
   }
-  finish_tiles(a, row, r, q, tiles, tile_slots, s, [&](float v, int32_t i) {
+  finish_tiles(a, row, r, q, tiles.count, tiles.slots, s, [&](float v, int32_t i) {
     const uint64_t x = w(v);
-    return v > -INFINITY && place_of(key_of(v), i) >= last && x >= least ? x : (uint64_t)0;
+    return v > -INFINITY && place_of(key_of(v), i) >= last_place && x >= least ? x : (uint64_t)0;
   });
 }
 
 int frac_bits(int64_t vocab) {
   int b = 0;
   while (((int64_t)1 << b) < vocab) ++b;
-  return 62 - b < 48 ? 62 - b : 48;
+  return 62 - b < 47 ? 62 - b : 47;  // (16 weights stay below 2^52)
 }
 
 }  // namespace
@@ -1100,7 +1540,7 @@ int64_t chunks_of(int64_t vocab, bool f32) {
 
 int64_t align16(int64_t n) { return (n + 15) / 16 * 16; }
 
-// Workspace: masses of chunks and bins (64 bits), then chunk and piece maxima and bin counts.
+// Workspace: masses and lists (64 bits), then counts and maxima.
 int64_t workspace_of(int64_t rows, int64_t chunks, SampleArgs* a, char* base) {
   const int64_t pieces = chunks * (kChunkElements / kPieceElements);
   int64_t at = 0;
@@ -1110,26 +1550,32 @@ int64_t workspace_of(int64_t rows, int64_t chunks, SampleArgs* a, char* base) {
     return here;
   };
   const int64_t chunk_mass = take(rows * chunks * 8), bin_mass = take(rows * kBins * 8),
-                chunk_max = take(rows * chunks * 4), piece_max = take(rows * pieces * 4),
-                bin_count = take(rows * kBins * 4);
+                tile_mass = take(rows * kMaxTiles * 8), list = take(rows * kList * 8),
+                list_count = take(rows * 4), chunk_max = take(rows * chunks * 4),
+                piece_max = take(rows * pieces * 4);
   if (a) {
     a->chunks = (int32_t)chunks;
     a->pieces = (int32_t)pieces;
     a->chunk_mass = reinterpret_cast<uint64_t*>(base + chunk_mass);
     a->bin_mass = reinterpret_cast<uint64_t*>(base + bin_mass);
+    a->tile_mass = reinterpret_cast<uint64_t*>(base + tile_mass);
+    a->list = reinterpret_cast<uint64_t*>(base + list);
+    a->list_count = reinterpret_cast<int32_t*>(base + list_count);
     a->chunk_max = reinterpret_cast<float*>(base + chunk_max);
     a->piece_max = reinterpret_cast<float*>(base + piece_max);
-    a->bin_count = reinterpret_cast<uint32_t*>(base + bin_count);
   }
   return at;
 }
 
 template <int DT>
 void launch_sample(const SampleArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL(chunk_kernel<DT>, dim3((unsigned)(a.rows * a.chunks)), dim3(kChunkThreads), 0,
-                     s, a);
-  if (a.parts > 0)
-    hipLaunchKernelGGL(bins_kernel<DT>, dim3((unsigned)(a.rows * a.parts)), dim3(kThreads), 0, s, a);
+  hipLaunchKernelGGL(chunk_kernel<DT>, dim3((unsigned)(a.rows * a.runs)), dim3(kChunkThreads), 0, s,
+                     a);
+  if (a.parts > 0) {
+    const dim3 grid((unsigned)(a.rows * a.parts));
+    hipLaunchKernelGGL(bins_kernel<DT>, grid, dim3(kThreads), 0, s, a);
+    hipLaunchKernelGGL(gather_kernel<DT>, grid, dim3(kThreads), 0, s, a);
+  }
   hipLaunchKernelGGL(row_kernel<DT>, dim3((unsigned)a.rows), dim3(kThreads), 0, s, a);
 }
 
@@ -1170,12 +1616,17 @@ extern "C" int int8kv_sample_rows(const void* logits, int logits_dtype, int64_t 
   a.out = out;
   hipStream_t s = static_cast<hipStream_t>(stream);
   workspace_of(rows, chunks_of(vocab, logits_dtype == INT8KV_F32), &a, static_cast<char*>(workspace));
-  // The histogram pass runs where some row may need it (a nucleus cut, whose mass is the whole
-  // row's; a large top-k alone is counted by its own row): about two workgroups per compute unit.
+  // Runs of chunks long enough for the loads of one to hide behind the weights of another, while
+  // there are enough of them to fill the compute units.
+  const int64_t per_unit = rows * a.chunks / 2048;
+  a.run_chunks = (int32_t)(per_unit < 1 ? 1 : (per_unit < 8 ? per_unit : 8));
+  a.runs = (a.chunks + a.run_chunks - 1) / a.run_chunks;
+  // The histogram pass and the gathering behind it run where some row may have a nucleus cut alone
+  // and more tokens than its list holds: about one workgroup per compute unit.
   a.parts = 0;
-  if (top_p) {
+  if (top_p && a.pieces > kList / kPieceElements) {
     const int64_t most = (vocab + 4 * kThreads - 1) / (4 * kThreads);
-    const int64_t want = 512 / rows < 1 ? 1 : 512 / rows;
+    const int64_t want = 256 / rows < 1 ? 1 : 256 / rows;
     a.parts = (int32_t)(want < most ? want : most);
   }
   if (logits_dtype == INT8KV_F32)
