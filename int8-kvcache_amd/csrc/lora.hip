@@ -29,7 +29,7 @@ constexpr int kMaxAdapters = 4096;
 constexpr int kMaxRank = 128;
 constexpr int64_t kMaxWidth = 1 << 20;
 constexpr int kPlanThreads = 1024;
-constexpr int kTileRows = 16;
+constexpr int kPlanTokens = 16;  // tokens per thread whose places stay in registers
 
 __device__ __forceinline__ float bf16_value(uint32_t h) { return __uint_as_float(h << 16); }
 __device__ __forceinline__ uint32_t bf16_bits(float f) {
@@ -37,16 +37,21 @@ __device__ __forceinline__ uint32_t bf16_bits(float f) {
 }
 
 // ------------------------------------------------------------------------------------ plan
-// int32 words: [0] tiles, [1] tokens with an adapter, [2..3] unused; the token of every position
-// (grouped by adapter, those without one last); adapter, first position and rows of every tile
-// (adapter -1: tokens without one).
+// {adapter, rows} of every tile (adapter -1: tokens without one; rows 0: an unused tile), then the
+// tokens of every tile, `tile` each (what lies behind its rows is not set).
 struct Plan {
-  int32_t* head;
-  int32_t* order;
-  int32_t* tile_adapter;
-  int32_t* tile_start;
-  int32_t* tile_rows;
+  int2* head;
+  int32_t* token;
+  int32_t tiles;  // at most
 };
+
+// Tokens per tile: 16 (one matrix tile), or 64 where the adapters have 32 tokens or more each: an
+// adapter's weights are then read for 64 tokens at a time (6007 tokens on 5 adapters, rank 64,
+// 3584 x 37888: 595 us with tiles of 16, most of it the traffic of B, 454 with 64 and nothing else
+// changed); below that the tiles would be mostly empty.
+int tile_rows(int64_t tokens, int32_t adapters) {
+  return tokens >= 32 * (int64_t)adapters && tokens >= 64 ? 64 : 16;
+}
 
 int64_t max_tiles(int64_t tokens, int32_t adapters, int rows) {
   const int64_t groups = (int64_t)adapters + 1 < tokens ? (int64_t)adapters + 1 : tokens;
@@ -54,14 +59,10 @@ int64_t max_tiles(int64_t tokens, int32_t adapters, int rows) {
 }
 
 Plan plan_at(const void* p, int64_t tokens, int32_t adapters) {
-  int32_t* w = static_cast<int32_t*>(const_cast<void*>(p));
-  const int64_t tiles = max_tiles(tokens, adapters, kTileRows);
   Plan q;
-  q.head = w;
-  q.order = w + 4;
-  q.tile_adapter = q.order + tokens;
-  q.tile_start = q.tile_adapter + tiles;
-  q.tile_rows = q.tile_start + tiles;
+  q.tiles = (int32_t)max_tiles(tokens, adapters, tile_rows(tokens, adapters));
+  q.head = static_cast<int2*>(const_cast<void*>(p));
+  q.token = reinterpret_cast<int32_t*>(q.head + (q.tiles + 1) / 2 * 2);
   return q;
 }
 
@@ -95,72 +96,63 @@ __device__ __forceinline__ int32_t plan_scan(int32_t v, int32_t* s_wave, int32_t
   return before + inc - v;
 }
 
-// Lanes of the wave with this lane's group: adds their number to *counter (one lane's atomic) and
-// returns this lane's place.  Neighbouring tokens mostly share their adapter.
-__device__ __forceinline__ int32_t take_place(int32_t group, bool valid, int32_t* counters) {
-  uint64_t todo = __ballot(valid);
-  int32_t place = 0;
-  const int lane = threadIdx.x & 63;
-  while (todo) {
-    const int leader = __ffsll((unsigned long long)todo) - 1;
-    const int32_t g = __shfl(group, leader, 64);
-    const uint64_t same = __ballot(valid && group == g);
-    int32_t at = 0;
-    if (lane == leader) at = atomicAdd(&counters[g], (int32_t)__popcll(same));
-    at = __shfl(at, leader, 64);
-    if (valid && group == g)
-      place = at + (int32_t)__popcll(same & (((uint64_t)1 << lane) - 1));
-    todo &= ~same;
-  }
-  return place;
-}
-
-// One workgroup: counts, offsets and places.  The order of tokens within a group may differ from
-// call to call; no result depends on it (a token's row is computed alike at every place).
-template <bool L64>
+// One workgroup: a token's place in its group from a counter in LDS, then the groups' first tiles.
+// The order of tokens within a group may differ from call to call; no result depends on it (a
+// token's row is computed alike at every place).  HELD: all places stay in registers; otherwise
+// they are counted a second time.
+template <bool L64, bool HELD>
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const void* ids, int32_t tokens,
                                                             int32_t adapters, int tile, Plan plan) {
   __shared__ int32_t s_count[kMaxAdapters + 1];
+  __shared__ int32_t s_tile[kMaxAdapters + 1];
   __shared__ int32_t s_wave[kPlanThreads / 64];
+  int32_t group[HELD ? kPlanTokens : 1], place[HELD ? kPlanTokens : 1];
+  if constexpr (HELD) {
+#pragma unroll
+    for (int j = 0; j < kPlanTokens; ++j) {
+      const int32_t t = j * kPlanThreads + (int32_t)threadIdx.x;
+      group[j] = t < tokens ? adapter_of<L64>(ids, t, adapters) : -1;
+    }
+  }
   for (int32_t g = threadIdx.x; g <= adapters; g += kPlanThreads) s_count[g] = 0;
   __syncthreads();
-  for (int32_t t0 = 0; t0 < tokens; t0 += kPlanThreads) {
-    const int32_t t = t0 + (int32_t)threadIdx.x;
-    const bool valid = t < tokens;
-    take_place(valid ? adapter_of<L64>(ids, t, adapters) : 0, valid, s_count);
+  if constexpr (HELD) {
+#pragma unroll
+    for (int j = 0; j < kPlanTokens; ++j)
+      if (group[j] >= 0) place[j] = atomicAdd(&s_count[group[j]], 1);
+  } else {
+    for (int32_t t = threadIdx.x; t < tokens; t += kPlanThreads)
+      atomicAdd(&s_count[adapter_of<L64>(ids, t, adapters)], 1);
   }
   __syncthreads();
-  // Offsets of the groups and of their tiles; each thread a contiguous span of groups.
+  // The groups' first tiles; each thread a contiguous span of groups.
   const int32_t per = (adapters + 1 + kPlanThreads - 1) / kPlanThreads;
   const int32_t g0 = (int32_t)threadIdx.x * per;
   const int32_t g1 = g0 + per < adapters + 1 ? g0 + per : adapters + 1;
-  int32_t rows = 0, tiles = 0;
-  for (int32_t g = g0; g < g1; ++g) {
-    rows += s_count[g];
-    tiles += (s_count[g] + tile - 1) / tile;
-  }
-  int32_t all_rows, all_tiles;
-  int32_t row = plan_scan(rows, s_wave, all_rows);
+  int32_t tiles = 0;
+  for (int32_t g = g0; g < g1; ++g) tiles += (s_count[g] + tile - 1) / tile;
+  int32_t all_tiles;
   int32_t at = plan_scan(tiles, s_wave, all_tiles);
   for (int32_t g = g0; g < g1; ++g) {
     const int32_t n = s_count[g];
-    for (int32_t i = 0; i < n; i += tile) {
-      plan.tile_adapter[at] = g < adapters ? g : -1;
-      plan.tile_start[at] = row + i;
-      plan.tile_rows[at] = n - i < tile ? n - i : tile;
-      ++at;
-    }
-    s_count[g] = row;  // now the group's next place
-    if (g == adapters) plan.head[1] = row;
-    row += n;
+    s_tile[g] = at;
+    for (int32_t i = 0; i < n; i += tile)
+      plan.head[at++] = int2{g < adapters ? g : -1, n - i < tile ? n - i : tile};
+    s_count[g] = 0;
   }
-  if (threadIdx.x == 0) plan.head[0] = all_tiles;
+  for (int32_t i = all_tiles + (int32_t)threadIdx.x; i < plan.tiles; i += kPlanThreads)
+    plan.head[i] = int2{-1, 0};
   __syncthreads();
-  for (int32_t t0 = 0; t0 < tokens; t0 += kPlanThreads) {
-    const int32_t t = t0 + (int32_t)threadIdx.x;
-    const bool valid = t < tokens;
-    const int32_t p = take_place(valid ? adapter_of<L64>(ids, t, adapters) : 0, valid, s_count);
-    if (valid) plan.order[p] = t;
+  if constexpr (HELD) {
+#pragma unroll
+    for (int j = 0; j < kPlanTokens; ++j)
+      if (group[j] >= 0)
+        plan.token[s_tile[group[j]] * tile + place[j]] = j * kPlanThreads + (int32_t)threadIdx.x;
+  } else {
+    for (int32_t t = threadIdx.x; t < tokens; t += kPlanThreads) {
+      const int32_t g = adapter_of<L64>(ids, t, adapters);
+      plan.token[s_tile[g] * tile + atomicAdd(&s_count[g], 1)] = t;
+    }
   }
 }
 
@@ -177,115 +169,261 @@ struct LoraArgs {
   const float* scales;
   uint16_t* out;
   int64_t out_stride;
-  float* part;  // [splits][tokens (in plan order)][rank]
+  float* part;  // [splits][tiles x rows of a tile][rank]
   Plan plan;
-  int32_t tokens, k, n, rank;
-  int32_t splits;   // parts of k
-  int32_t chunk;    // k of a part (a multiple of 32)
-  int32_t chunks;   // column chunks of the second product
+  int32_t k, n, rank;
+  int32_t splits;  // parts of k
+  int32_t chunk;   // k of a part (a multiple of 32)
+  int32_t halves;  // parts of the rank, 64 each (first product)
+  int32_t chunks;  // column chunks (second product), taken in `groups` of `run`
+  int32_t groups, run;
 };
 
 __device__ __forceinline__ bf16x8 load8(const uint16_t* p) {
   return __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(p));
 }
+// 16 bytes of base or out; STREAM: past the caches.
+template <bool STREAM>
+__device__ __forceinline__ u32x4 load16(const uint16_t* p) {
+  if constexpr (STREAM) return __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+  return *reinterpret_cast<const u32x4*>(p);
+}
+template <bool STREAM>
+__device__ __forceinline__ void store16(uint16_t* p, u32x4 v) {
+  if constexpr (STREAM)
+    __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(p));
+  else
+    *reinterpret_cast<u32x4*>(p) = v;
+}
 __device__ __forceinline__ bf16x8 zero8() {
   return __builtin_bit_cast(bf16x8, u32x4{0u, 0u, 0u, 0u});
 }
 
-// x A^T of one tile and one part of k.  Four waves take the part's 32-wide steps in turn; RT:
-// 16-row tiles of A.  Operands straight from memory: lane (i, g) holds 8 consecutive k of row i.
-constexpr int kShrinkWaves = 4;
-template <int RT>
-__global__ __launch_bounds__(kShrinkWaves * 64) void shrink_kernel(LoraArgs a) {
-  __shared__ f32x4 s_acc[kShrinkWaves][RT][64];
-  const int32_t tile = blockIdx.x / a.splits;
-  const int32_t split = blockIdx.x - tile * a.splits;
-  if (tile >= a.plan.head[0]) return;
-  const int32_t adapter = a.plan.tile_adapter[tile];
-  if (adapter < 0) return;
-  const int32_t start = a.plan.tile_start[tile];
-  const int32_t rows = a.plan.tile_rows[tile];
+// x A^T of one tile (TT x 16 tokens), one part of k and at most 64 ranks (RT x 16).  The waves
+// take the part's 32-wide steps in turn, each with its next step's operands in flight, and add up
+// through LDS.  Operands straight from memory: lane (i, g) holds 8 consecutive k of row i.
+template <int TT>
+constexpr int kShrinkWaves = TT == 1 ? 4 : 8;
+template <int TT, int RT>
+__global__ __launch_bounds__(kShrinkWaves<TT> * 64) void shrink_kernel(LoraArgs a) {
+  constexpr int kRows = 16 * TT;
+  constexpr int kWaves = kShrinkWaves<TT>;
+  __shared__ f32x4 s_acc[kWaves / 2][TT * RT][64];
+  const int32_t per_tile = a.splits * a.halves;
+  const int32_t tile = blockIdx.x / per_tile;
+  const int32_t rest = blockIdx.x - tile * per_tile;
+  const int32_t split = rest / a.halves;
+  const int32_t r0 = 64 * (rest - split * a.halves);
   const int lane = threadIdx.x & 63;
-  const int wave = threadIdx.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i = lane & 15;
   const int g = lane >> 4;
-  const int32_t token = a.plan.order[start + (i < rows ? i : rows - 1)];
-  const uint16_t* xp = a.x + token * a.x_stride + 8 * g;
+  const int2 head = a.plan.head[tile];
+  int32_t token[TT];
+#pragma unroll
+  for (int tt = 0; tt < TT; ++tt) token[tt] = a.plan.token[tile * kRows + 16 * tt + i];
+  const int32_t adapter = __builtin_amdgcn_readfirstlane(head.x);
+  const int32_t rows = __builtin_amdgcn_readfirstlane(head.y);
+  if (adapter < 0) return;  // (unused tiles too)
+  const int32_t first = __builtin_amdgcn_readlane(token[0], 0);
+  const uint16_t* xp[TT];
+#pragma unroll
+  for (int tt = 0; tt < TT; ++tt)
+    xp[tt] = a.x + (int64_t)(16 * tt + i < rows ? token[tt] : first) * a.x_stride + 8 * g;
   const uint16_t* ap[RT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    const int32_t r = 16 * rt + i;
+    const int32_t r = r0 + 16 * rt + i;
     ap[rt] = a.a + adapter * a.a_adapter + (int64_t)(r < a.rank ? r : a.rank - 1) * a.a_row + 8 * g;
   }
-  f32x4 acc[RT];
+  f32x4 acc[TT][RT];
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) acc[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) acc[tt][rt] = f32x4{0.f, 0.f, 0.f, 0.f};
   const int32_t k0 = split * a.chunk;
   const int32_t k1 = k0 + a.chunk < a.k ? k0 + a.chunk : a.k;
-  for (int32_t k = k0 + 32 * wave; k < k1; k += 32 * kShrinkWaves) {
+  // Steps in flight: as many as leave the tile's operands room in the registers.
+  constexpr int kFlight = TT * RT == 1 ? 4 : (TT * RT <= 4 ? 2 : 1);
+  constexpr int kStep = 32 * kWaves;
+  bf16x8 xv[kFlight][TT], av[kFlight][RT];
+  const auto request = [&](int f, int32_t k) {
     const bool in = k + 8 * g < k1;  // k is a multiple of 8
-    const bf16x8 xv = in ? load8(xp + k) : zero8();
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const bf16x8 av = in ? load8(ap[rt] + k) : zero8();
-      acc[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, xv, acc[rt], 0, 0, 0);
+    for (int tt = 0; tt < TT; ++tt) xv[f][tt] = in ? load8(xp[tt] + k) : zero8();
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) av[f][rt] = in ? load8(ap[rt] + k) : zero8();
+  };
+  int32_t k = k0 + 32 * wave;
+#pragma unroll
+  for (int f = 0; f < kFlight; ++f) request(f, k + f * kStep);
+  for (; k < k1; k += kFlight * kStep) {
+#pragma unroll
+    for (int f = 0; f < kFlight; ++f) {
+      bf16x8 x[TT], w[RT];
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt) x[tt] = xv[f][tt];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) w[rt] = av[f][rt];
+      request(f, k + (kFlight + f) * kStep);
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+          acc[tt][rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[rt], x[tt], acc[tt][rt], 0, 0, 0);
     }
   }
+  // The upper half of the waves hands its sums to the lower half, until wave 0 has all.
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) s_acc[wave][rt][lane] = acc[rt];
-  __syncthreads();
-  // Lane (i, g) of tile rt: ranks 16 rt + 4 g .. + 3 of token i.
-  for (int rt = wave; rt < RT; rt += kShrinkWaves) {
-    f32x4 y = s_acc[0][rt][lane];
+  for (int half = kWaves / 2; half >= 1; half >>= 1) {
+    if (wave >= half && wave < 2 * half)
 #pragma unroll
-    for (int w = 1; w < kShrinkWaves; ++w) y += s_acc[w][rt][lane];
-    const int32_t r = 16 * rt + 4 * g;
-    if (i < rows && r < a.rank)
-      *reinterpret_cast<f32x4*>(a.part + ((int64_t)split * a.tokens + start + i) * a.rank + r) = y;
+      for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) s_acc[wave - half][tt * RT + rt][lane] = acc[tt][rt];
+    __syncthreads();
+    if (wave < half)
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) acc[tt][rt] += s_acc[wave][tt * RT + rt][lane];
+    __syncthreads();
   }
+  // Lane (i, g) of tile (tt, rt): ranks 16 rt + 4 g .. + 3 of token 16 tt + i.
+  if (wave == 0)
+#pragma unroll
+    for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const int32_t r = r0 + 16 * rt + 4 * g;
+        const int64_t row = ((int64_t)split * a.plan.tiles + tile) * kRows + 16 * tt + i;
+        if (16 * tt + i < rows && r < a.rank)
+          *reinterpret_cast<f32x4*>(a.part + row * a.rank + r) = acc[tt][rt];
+      }
 }
 
 // The second product of one tile and one chunk of columns.  The rank-wide vectors are staged in
 // LDS as two bf16 parts, upper (truncated: no overflow) and rest; along the product's inner axis
-// first all upper parts, then all rests, against the same row of B.
+// first all upper parts, then all rests, against the same row of B.  NS: 32-wide steps of that
+// axis; PAIRED: the rank is a multiple of 32, and the second half of the steps meets the first
+// half's operands of B.  B's operands stay in registers for all tokens of the tile.
+// Tiles of 64 tokens: a workgroup takes a run of column chunks, so that the vectors are read for
+// more than 256 columns, and the workgroups of one die (every eighth) take the same columns of all
+// tiles in turn, so that B is read into one L2 cache only.
+// Loads are requested as early as their addresses are known: the partial sums (which depend on the
+// tile's number alone), then B and the first base rows.  Base and out are read and written in
+// whole 128-byte lines, eight lanes each; the products get there through LDS (in operand order,
+// where neighbouring lanes hold different rows, 6007 x 37888 took 437 us instead of 365).
 constexpr int kExpandWaves = 4;
 constexpr int kWaveColumns = 64;
 constexpr int kExpandColumns = kExpandWaves * kWaveColumns;
-template <int RT>
+constexpr int kXcds = 8;
+constexpr int64_t kInfinityCacheBytes = 256 << 20;  // base and out beyond it stream past the caches
+template <int TT, int NS, bool PAIRED, bool STREAM>
 __global__ __launch_bounds__(kExpandWaves * 64) void expand_kernel(LoraArgs a) {
+  constexpr int kRows = 16 * TT;
   constexpr int kPad = 8;
-  __shared__ __align__(16) uint16_t s_h[kTileRows][2 * 16 * RT + kPad];
-  const int32_t tile = blockIdx.x / a.chunks;
-  const int32_t chunk = blockIdx.x - tile * a.chunks;
-  if (tile >= a.plan.head[0]) return;
-  const int32_t adapter = a.plan.tile_adapter[tile];
-  const int32_t start = a.plan.tile_start[tile];
-  const int32_t rows = a.plan.tile_rows[tile];
+  constexpr int kHeld = PAIRED ? NS / 2 : NS;
+  __shared__ __align__(16) uint16_t s_h[kRows][32 * NS + kPad];
+  __shared__ __align__(16) float s_out[kExpandWaves][16][kWaveColumns + 4];
+  __shared__ __align__(16) float s_way[TT == 1 ? 4 * kExpandWaves * 64 : 4];
+  int32_t tile, group;
+  if constexpr (TT == 1) {
+    tile = blockIdx.x / a.groups;
+    group = blockIdx.x - tile * a.groups;
+  } else {
+    const int32_t at = blockIdx.x / kXcds;
+    const int32_t round = at / a.plan.tiles;
+    tile = at - round * a.plan.tiles;
+    group = round * kXcds + blockIdx.x % kXcds;
+    if (group >= a.groups) return;
+  }
+  const int32_t chunk0 = group * a.run;
+  const int32_t chunk1 = chunk0 + a.run < a.chunks ? chunk0 + a.run : a.chunks;
   const int lane = threadIdx.x & 63;
-  const int wave = threadIdx.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i = lane & 15;
   const int g = lane >> 4;
+  const int2 head = a.plan.head[tile];
+  // As an operand lane (i, g) holds token i; in base and out lane l holds columns 8 (l % 8) .. + 7
+  // of rows l / 8 and 8 + l / 8.
+  const int line = lane >> 3;
+  int32_t token[TT][2];
+#pragma unroll
+  for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) token[tt][h] = a.plan.token[tile * kRows + 16 * tt + 8 * h + line];
+  // The tile's vectors, four values per thread and round (those behind its rows are not set; they
+  // meet no other row).
+  const int32_t quads = a.rank / 4;
+  const int64_t split_stride = (int64_t)a.plan.tiles * kRows * a.rank;
+  const float* part = a.part + (int64_t)tile * kRows * a.rank;
+  constexpr int kTogether = 8;  // partial sums requested together
+  f32x4 y[kTogether];
+  // Tiles of 16 have fewer values than threads: then thread (p, way) adds every ways-th sum of p.
+  const int32_t ways = TT == 1 && kRows * quads <= kExpandWaves * 32 ? kExpandWaves * 64 / (kRows * quads) : 1;
+  const int32_t way = ways > 1 ? (int32_t)threadIdx.x / (kRows * quads) : 0;
+  const int32_t p0 = (int32_t)threadIdx.x - way * kRows * quads;
+  const auto request_parts = [&](int32_t p, int32_t s0) {
+#pragma unroll
+    for (int u = 0; u < kTogether; ++u) {
+      const int32_t s = s0 + u * ways;
+      y[u] = *reinterpret_cast<const f32x4*>(part + (s < a.splits ? s : 0) * split_stride +
+                                             4 * (p < kRows * quads ? p : 0));
+    }
+  };
+  request_parts(p0, way);
+  const int32_t adapter = __builtin_amdgcn_readfirstlane(head.x);
+  const int32_t rows = __builtin_amdgcn_readfirstlane(head.y);
+  if (rows == 0) return;
   if (adapter < 0) {
     if (a.out == a.base && a.out_stride == a.base_stride) return;
-    const int32_t c0 = chunk * kExpandColumns;
-    const int32_t c1 = c0 + kExpandColumns < a.n ? c0 + kExpandColumns : a.n;
+    const int32_t c0 = chunk0 * kExpandColumns;
+    const int32_t c1 = chunk1 * kExpandColumns < a.n ? chunk1 * kExpandColumns : a.n;
     const int32_t pieces = (c1 - c0) / 8;
     for (int32_t p = threadIdx.x; p < rows * pieces; p += kExpandWaves * 64) {
       const int32_t r = p / pieces;
-      const int64_t t = a.plan.order[start + r];
+      const int64_t t = a.plan.token[tile * kRows + r];
       const int32_t c = c0 + 8 * (p - r * pieces);
       *reinterpret_cast<u32x4*>(a.out + t * a.out_stride + c) =
           *reinterpret_cast<const u32x4*>(a.base + t * a.base_stride + c);
     }
     return;
   }
-  const int32_t quads = a.rank / 4;
-  for (int32_t p = threadIdx.x; p < rows * quads; p += kExpandWaves * 64) {
+  const int32_t first = __builtin_amdgcn_readlane(token[0][0], 0);
+  const int32_t granules = a.rank / 8;  // 8-wide pieces of one part
+  int32_t col0 = chunk0 * kExpandColumns + wave * kWaveColumns;
+  int32_t col = col0 + 8 * (lane & 7);  // this lane's in base and out
+  bool in = col < a.n;
+  u32x4 base[TT][2];  // of all the tile's tokens: requested a chunk ahead
+  const auto request_base = [&](int tt) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int64_t t = 16 * tt + 8 * h + line < rows ? token[tt][h] : first;
+      base[tt][h] = in ? load16<STREAM>(a.base + t * a.base_stride + col) : u32x4{0u, 0u, 0u, 0u};
+    }
+  };
+#pragma unroll
+  for (int tt = 0; tt < TT; ++tt) request_base(tt);
+  // Row 4 g + r of matrix tile j's operand is column 16 j + 4 g + r.
+  bf16x8 bv[kHeld][4];
+  const auto request_b = [&]() {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int32_t c = col0 + 16 * j + i;
+      const uint16_t* bp = a.b + adapter * a.b_adapter + (int64_t)(c < a.n ? c : a.n - 1) * a.b_row;
+#pragma unroll
+      for (int s = 0; s < kHeld; ++s) {
+        const int32_t p = 4 * s + g;
+        bv[s][j] = p < 2 * granules ? load8(bp + 8 * (p < granules ? p : p - granules)) : zero8();
+      }
+    }
+  };
+  request_b();
+  const float scale = a.scales ? a.scales[adapter] : 1.0f;
+  const auto stage = [&](int32_t p, f32x4 h) {
     const int32_t r = p / quads;
     const int32_t c = 4 * (p - r * quads);
-    f32x4 h = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int32_t s = 0; s < a.splits; ++s)
-      h += *reinterpret_cast<const f32x4*>(a.part + ((int64_t)s * a.tokens + start + r) * a.rank + c);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const uint32_t hi = __float_as_uint(h[j]) >> 16;
@@ -293,51 +431,73 @@ __global__ __launch_bounds__(kExpandWaves * 64) void expand_kernel(LoraArgs a) {
       s_h[r][c + j] = (uint16_t)hi;
       s_h[r][a.rank + c + j] = fabsf(h[j]) < INFINITY ? (uint16_t)bf16_bits(rest) : 0;
     }
+  };
+  for (int32_t p = p0; p < kRows * quads; p += kExpandWaves * 64) {
+    f32x4 h = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int32_t s0 = way; s0 < a.splits; s0 += kTogether * ways) {
+      if (p != p0 || s0 != way) request_parts(p, s0);
+#pragma unroll
+      for (int u = 0; u < kTogether; ++u)
+        if (s0 + u * ways < a.splits) h += y[u];
+    }
+    if (ways == 1)
+      stage(p, h);
+    else if (way < ways)
+      *reinterpret_cast<f32x4*>(&s_way[4 * threadIdx.x]) = h;
+  }
+  if (ways > 1) {
+    __syncthreads();
+    if ((int32_t)threadIdx.x < kRows * quads) {
+      f32x4 h = *reinterpret_cast<const f32x4*>(&s_way[4 * threadIdx.x]);
+      for (int32_t w = 1; w < ways; ++w)
+        h += *reinterpret_cast<const f32x4*>(&s_way[4 * (threadIdx.x + w * kRows * quads)]);
+      stage(threadIdx.x, h);
+    }
   }
   __syncthreads();
-  // Columns of this wave: lane g's 16 consecutive ones, 4 per matrix tile j (row 4 g + r of tile
-  // j's operand is column 16 g + 4 j + r), so a token's 64 columns are one 128-byte line.
-  const int32_t col0 = chunk * kExpandColumns + wave * kWaveColumns;
-  if (col0 >= a.n) return;
-  const uint16_t* bp[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int32_t c = col0 + 16 * (i >> 2) + 4 * j + (i & 3);
-    bp[j] = a.b + adapter * a.b_adapter + (int64_t)(c < a.n ? c : a.n - 1) * a.b_row;
-  }
-  f32x4 acc[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const int32_t granules = a.rank / 8;  // 8-wide pieces of one part
-  const int row = i < rows ? i : rows - 1;
-  for (int32_t s = 0; s < 2 * granules; s += 4) {
-    const int32_t p = s + g;
-    const bool in = p < 2 * granules;
-    const int32_t at = p < granules ? p : p - granules;
-    const bf16x8 hv = in ? load8(&s_h[row][8 * p]) : zero8();
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const bf16x8 bv = in ? load8(bp[j] + 8 * at) : zero8();
-      acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bv, hv, acc[j], 0, 0, 0);
+  for (int32_t chunk = chunk0; chunk < chunk1; ++chunk) {
+    if (chunk > chunk0) request_b();
+    const int32_t here = col;
+    const bool in_here = in;
+    if (chunk + 1 < chunk1) {
+      col0 += kExpandColumns;
+      col += kExpandColumns;
+      in = col < a.n;
     }
-  }
-  if (i >= rows) return;
-  const int64_t t = a.plan.order[start + i];
-  const float scale = a.scales ? a.scales[adapter] : 1.0f;
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int32_t c = col0 + 16 * g + 8 * half;
-    if (c >= a.n) break;
-    const u32x4 v = *reinterpret_cast<const u32x4*>(a.base + t * a.base_stride + c);
-    u32x4 o;
+    for (int tt = 0; tt < TT; ++tt) {
+      if (16 * tt >= rows) break;  // (uniform)
+      const u32x4 v[2] = {base[tt][0], base[tt][1]};
+      if (chunk + 1 < chunk1) request_base(tt);
+      f32x4 acc[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const f32x4 d = acc[2 * half + (j >> 1)];
-      const float lo = d[2 * (j & 1)] * scale + bf16_value(v[j] & 0xffffu);
-      const float hi = d[2 * (j & 1) + 1] * scale + bf16_value(v[j] >> 16);
-      o[j] = bf16_bits(lo) | (bf16_bits(hi) << 16);
+      for (int j = 0; j < 4; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        const int32_t p = 4 * s + g;
+        const bf16x8 hv = p < 2 * granules ? load8(&s_h[16 * tt + i][8 * p]) : zero8();
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bv[s % kHeld][j], hv, acc[j], 0, 0, 0);
+      }
+      // (The wave's own buffer, and a wave's LDS accesses run in order: no barrier.)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) *reinterpret_cast<f32x4*>(&s_out[wave][i][16 * j + 4 * g]) = acc[j];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float* q = &s_out[wave][8 * h + line][8 * (lane & 7)];
+        const f32x4 d[2] = {*reinterpret_cast<const f32x4*>(q), *reinterpret_cast<const f32x4*>(q + 4)};
+        u32x4 o;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float lo = d[j >> 1][2 * (j & 1)] * scale + bf16_value(v[h][j] & 0xffffu);
+          const float hi = d[j >> 1][2 * (j & 1) + 1] * scale + bf16_value(v[h][j] >> 16);
+          o[j] = bf16_bits(lo) | (bf16_bits(hi) << 16);
+        }
+        if (in_here && 16 * tt + 8 * h + line < rows)
+          store16<STREAM>(a.out + (int64_t)token[tt][h] * a.out_stride + here, o);
+      }
     }
-    *reinterpret_cast<u32x4*>(a.out + t * a.out_stride + c) = o;
   }
 }
 
@@ -345,11 +505,19 @@ bool rows16(const void* p, int64_t stride) {
   return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && stride % 8 == 0;
 }
 
-int splits_for(int64_t tiles, int64_t k) {
-  const int64_t steps = (k + 127) / 128;
-  int64_t s = (512 + tiles - 1) / (tiles > 0 ? tiles : 1);
-  s = s < 1 ? 1 : (s > 8 ? 8 : s);
-  return (int)(s < steps ? s : steps);
+// Parts of k.  Tiles of 16 tokens: about four workgroups of four waves per compute unit (32 tokens
+// on 24 adapters, the four projections of a layer: 35 us with 12-16 parts, 37 with 8, 56 with 2).
+// Tiles of 64: eight waves, about 1.5 workgroups per unit (34 tiles, 18944 x 3584: 26 us with 12
+// parts, 31 with 6, 29 with 16); from 64 tiles on no parts below 1536, since every workgroup of
+// the second product reads all parts of its tile (99 tiles, 3584 x 37888: 239 us with 2, 250 with
+// 4).  A part has at least two steps per wave.
+int splits_for(int64_t tiles, int64_t k, int rows) {
+  const int64_t shortest = rows == 16 ? 2 * 32 * kShrinkWaves<1>
+                                      : (tiles >= 64 ? 1536 : 2 * 32 * kShrinkWaves<4>);
+  const int64_t most = k / shortest;
+  int64_t s = ((rows == 16 ? 1024 : 384) + tiles - 1) / (tiles > 0 ? tiles : 1);
+  s = s < most ? s : most;
+  return (int)(s < 1 ? 1 : (s < 16 ? s : 16));
 }
 
 bool lora_sizes_ok(int64_t tokens, int32_t adapters, int64_t k, int32_t rank) {
@@ -357,12 +525,56 @@ bool lora_sizes_ok(int64_t tokens, int32_t adapters, int64_t k, int32_t rank) {
          k >= 8 && k % 8 == 0 && k <= kMaxWidth && rank >= 8 && rank % 8 == 0 && rank <= kMaxRank;
 }
 
-template <int RT>
-void launch_lora(const LoraArgs& a, int64_t tiles, hipStream_t s) {
-  hipLaunchKernelGGL(shrink_kernel<RT>, dim3((unsigned)(tiles * a.splits)),
-                     dim3(kShrinkWaves * 64), 0, s, a);
-  hipLaunchKernelGGL(expand_kernel<RT>, dim3((unsigned)(tiles * a.chunks)),
-                     dim3(kExpandWaves * 64), 0, s, a);
+template <int TT>
+void launch_shrink(const LoraArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)((int64_t)a.plan.tiles * a.splits * a.halves)), block(kShrinkWaves<TT> * 64);
+  if (a.rank <= 16)
+    hipLaunchKernelGGL((shrink_kernel<TT, 1>), grid, block, 0, s, a);
+  else if (a.rank <= 32)
+    hipLaunchKernelGGL((shrink_kernel<TT, 2>), grid, block, 0, s, a);
+  else
+    hipLaunchKernelGGL((shrink_kernel<TT, 4>), grid, block, 0, s, a);
+}
+
+template <int TT, bool STREAM>
+void launch_expand(const LoraArgs& a, hipStream_t s) {
+  const int64_t groups = TT == 1 ? a.groups : (a.groups + kXcds - 1) / kXcds * kXcds;
+  const dim3 grid((unsigned)(a.plan.tiles * groups)), block(kExpandWaves * 64);
+  const bool paired = a.rank % 32 == 0;
+  switch ((2 * a.rank + 31) / 32) {
+#define INT8KV_EXPAND(NS, PAIRED) \
+  hipLaunchKernelGGL((expand_kernel<TT, NS, PAIRED, STREAM>), grid, block, 0, s, a)
+    case 1: INT8KV_EXPAND(1, false); break;
+    case 2:
+      if (paired)
+        INT8KV_EXPAND(2, true);
+      else
+        INT8KV_EXPAND(2, false);
+      break;
+    case 3: INT8KV_EXPAND(3, false); break;
+    case 4:
+      if (paired)
+        INT8KV_EXPAND(4, true);
+      else
+        INT8KV_EXPAND(4, false);
+      break;
+    case 5: INT8KV_EXPAND(5, false); break;
+    case 6:
+      if (paired)
+        INT8KV_EXPAND(6, true);
+      else
+        INT8KV_EXPAND(6, false);
+      break;
+    case 7: INT8KV_EXPAND(7, false); break;
+    case 8:
+      if (paired)
+        INT8KV_EXPAND(8, true);
+      else
+        INT8KV_EXPAND(8, false);
+      break;
+#undef INT8KV_EXPAND
+    default: break;
+  }
 }
 
 }  // namespace
@@ -372,7 +584,9 @@ using namespace int8kv_serving;
 
 extern "C" size_t int8kv_lora_plan_bytes(int64_t tokens, int32_t num_adapters) {
   if (tokens < 0 || tokens > kMaxTokens || num_adapters < 1 || num_adapters > kMaxAdapters) return 0;
-  return 4 * (size_t)(4 + tokens + 3 * max_tiles(tokens, num_adapters, kTileRows));
+  const int rows = tile_rows(tokens, num_adapters);
+  const int64_t tiles = max_tiles(tokens, num_adapters, rows);
+  return 16 + 8 * (size_t)((tiles + 1) / 2 * 2) + 4 * (size_t)(tiles * rows);
 }
 
 extern "C" int int8kv_lora_plan(const void* adapter_ids, int ids_dtype, int64_t tokens,
@@ -384,17 +598,20 @@ extern "C" int int8kv_lora_plan(const void* adapter_ids, int ids_dtype, int64_t 
   if (plan_bytes < need || reinterpret_cast<uintptr_t>(plan) % 16) return INT8KV_E_WORKSPACE;
   hipStream_t s = static_cast<hipStream_t>(stream);
   const Plan p = plan_at(plan, tokens, num_adapters);
-  auto kernel = ids_dtype == INT8KV_I64 ? plan_kernel<true> : plan_kernel<false>;
+  const bool held = tokens <= kPlanTokens * kPlanThreads;
+  auto kernel = ids_dtype == INT8KV_I64 ? (held ? plan_kernel<true, true> : plan_kernel<true, false>)
+                                        : (held ? plan_kernel<false, true> : plan_kernel<false, false>);
   hipLaunchKernelGGL(kernel, dim3(1), dim3(kPlanThreads), 0, s, adapter_ids, (int32_t)tokens,
-                     num_adapters, kTileRows, p);
+                     num_adapters, tile_rows(tokens, num_adapters), p);
   return (int)hipGetLastError();
 }
 
 extern "C" size_t int8kv_lora_workspace_bytes(int64_t tokens, int32_t num_adapters, int64_t k,
                                               int32_t rank) {
   if (!lora_sizes_ok(tokens, num_adapters, k, rank)) return 0;
-  const int64_t tiles = max_tiles(tokens, num_adapters, kTileRows);
-  return (size_t)(tokens > 0 ? tokens : 1) * rank * 4 * splits_for(tiles, k);
+  const int rows = tile_rows(tokens, num_adapters);
+  const int64_t tiles = max_tiles(tokens, num_adapters, rows);
+  return 16 + (size_t)tiles * rows * rank * 4 * splits_for(tiles, k, rows);
 }
 
 extern "C" int int8kv_lora_add(const void* base, int64_t base_row_stride, const void* x,
@@ -440,24 +657,31 @@ extern "C" int int8kv_lora_add(const void* base, int64_t base_row_stride, const 
   a.out_stride = out_row_stride;
   a.part = static_cast<float*>(workspace);
   a.plan = plan_at(plan, tokens, num_adapters);
-  a.tokens = (int32_t)tokens;
   a.k = (int32_t)k;
   a.n = (int32_t)n;
   a.rank = rank;
-  const int64_t tiles = max_tiles(tokens, num_adapters, kTileRows);
-  a.splits = splits_for(tiles, k);
+  const int64_t tiles = a.plan.tiles;
+  const int rows = tile_rows(tokens, num_adapters);
+  a.splits = splits_for(tiles, k, rows);
   a.chunk = (int32_t)(((k + a.splits - 1) / a.splits + 31) / 32 * 32);
+  a.halves = (rank + 63) / 64;
   a.chunks = (int32_t)((n + kExpandColumns - 1) / kExpandColumns);
-  if (tiles * a.chunks > 0x7fffffff) return INT8KV_E_SHAPE;
+  // Runs of chunks: while there are about fourteen workgroups per compute unit (99 tiles of 148
+  // chunks: runs of 4 240 us, 2 255, 8 265, 1 300).
+  int64_t run = rows == 16 ? 1 : tiles * a.chunks / 3584;
+  a.run = (int32_t)(run < 1 ? 1 : (run < 8 ? run : 8));
+  a.groups = (a.chunks + a.run - 1) / a.run;
+  if (tiles * (a.groups + kXcds) > 0x7fffffff) return INT8KV_E_SHAPE;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const int tiles_of_rank = (rank + 15) / 16;
-  if (tiles_of_rank <= 1)
-    launch_lora<1>(a, tiles, s);
-  else if (tiles_of_rank <= 2)
-    launch_lora<2>(a, tiles, s);
-  else if (tiles_of_rank <= 4)
-    launch_lora<4>(a, tiles, s);
-  else
-    launch_lora<8>(a, tiles, s);
+  if (rows == 64) {
+    launch_shrink<4>(a, s);
+    if (4 * tokens * n > kInfinityCacheBytes)
+      launch_expand<4, true>(a, s);
+    else
+      launch_expand<4, false>(a, s);
+  } else {
+    launch_shrink<1>(a, s);
+    launch_expand<1, false>(a, s);
+  }
   return (int)hipGetLastError();
 }

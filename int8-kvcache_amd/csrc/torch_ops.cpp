@@ -350,7 +350,26 @@ void build_batch_tables(at::Tensor computed_lens, at::Tensor new_lens, const at:
   check_status(st, "int8kv_batch_tables");
 }
 
-// int8kv/lora.py (the same checks).
+// int8kv/lora.py (the same checks): fills `plan`, or a new buffer.
+at::Tensor lora_plan(at::Tensor adapter_ids, int64_t num_adapters, c10::optional<at::Tensor> plan) {
+  require(adapter_ids.dim() == 1 && is_index(adapter_ids.scalar_type()));
+  require(num_adapters >= 1 && num_adapters <= 4096, "num_adapters must lie in [1, 4096]");
+  require(adapter_ids.is_cuda(), "lora_plan needs GPU tensors");
+  const int64_t tokens = adapter_ids.numel();
+  require(tokens <= (1 << 24), "at most 2^24 tokens");
+  adapter_ids = adapter_ids.contiguous();
+  const c10::hip::HIPGuard guard(adapter_ids.device().index());
+  if (!plan.has_value())
+    plan = at::empty({(int64_t)int8kv_lora_plan_bytes(tokens, (int32_t)num_adapters)},
+                     adapter_ids.options().dtype(at::kByte));
+  require_same_device({&*plan}, adapter_ids);
+  const int st = int8kv_lora_plan(adapter_ids.data_ptr(), dtype_code(adapter_ids.scalar_type()),
+                                  tokens, (int32_t)num_adapters, plan->data_ptr(),
+                                  (size_t)plan->numel(), current_stream(adapter_ids));
+  check_status(st, "int8kv_lora_plan");
+  return *plan;
+}
+
 at::Tensor lora_add(const at::Tensor& base, const at::Tensor& x, const at::Tensor& lora_a,
                     const at::Tensor& lora_b, const at::Tensor& plan, int64_t plan_tokens,
                     int64_t plan_adapters, c10::optional<at::Tensor> scales,
@@ -464,6 +483,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("v_scale"), py::arg("out"), py::arg("num_ranges"), py::arg("flags"),
         py::arg("workspace"), py::arg("min_tiles"));
   m.def("build_batch_tables", &build_batch_tables);
+  m.def("lora_plan", &lora_plan);
   m.def("lora_add", &lora_add);
   m.def("sample_tokens", &sample_tokens);
   m.def("set_library_error", &set_library_error);

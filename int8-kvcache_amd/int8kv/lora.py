@@ -33,6 +33,13 @@ class LoraPlan:
 def lora_plan(adapter_ids: torch.Tensor, num_adapters: int, plan: LoraPlan | None = None) -> LoraPlan:
     """Groups the tokens of a step by adapter (int32 or int64 ids [tokens]; an id outside
     [0, num_adapters) means none).  ``plan``: an earlier plan of the same sizes to fill again."""
+    if plan is not None:
+        assert (plan.tokens, plan.num_adapters) == (adapter_ids.numel(), num_adapters), \
+            "a plan of other sizes"
+    ext = _ext.module()
+    if ext is not None:
+        buffer = ext.lora_plan(adapter_ids, num_adapters, None if plan is None else plan.buffer)
+        return plan if plan is not None else LoraPlan(buffer, adapter_ids.numel(), num_adapters)
     assert adapter_ids.dim() == 1 and adapter_ids.dtype in (torch.int32, torch.int64)
     assert 1 <= num_adapters <= MAX_ADAPTERS, "num_adapters must lie in [1, 4096]"
     assert adapter_ids.is_cuda, "lora_plan needs GPU tensors"
@@ -43,7 +50,6 @@ def lora_plan(adapter_ids: torch.Tensor, num_adapters: int, plan: LoraPlan | Non
     need = lib.int8kv_lora_plan_bytes(tokens, num_adapters)
     if plan is None:
         plan = LoraPlan(torch.empty(need, dtype=torch.uint8, device=dev), tokens, num_adapters)
-    assert (plan.tokens, plan.num_adapters) == (tokens, num_adapters), "a plan of other sizes"
     assert plan.buffer.device == dev, "all tensors must be on one device (the GPU)"
     with torch.cuda.device(dev):
         status = lib.int8kv_lora_plan(ids.data_ptr(), _lib.DTYPE_CODE[ids.dtype], tokens,
