@@ -6,23 +6,24 @@
 // no entry that another token writes (a new block's id comes from the free list itself), so
 // nothing has to wait for anything.
 //
-// Bound: latency.  A decode step of 32 requests moves 1.3 KB, and even a prefill of a million
-// tokens writes 20 bytes per token.  Up to kOneLaunch requests every workgroup scans all lengths
-// itself (in LDS) instead of a scan kernel running first: one launch.
+// Bound: latency (a decode step of 32 requests moves 1.3 KB), or the 20 bytes written per token of
+// a large prefill.  Up to kMostScanned requests every workgroup scans all lengths itself, one or
+// two requests per thread, instead of a scan kernel running first: one launch.
 
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
 
 #include "serving_ops.h"
+#include "wave_scan.h"
 
 namespace int8kv_serving {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kOneLaunch = 2048;  // requests whose prefix sums a workgroup keeps in LDS (40 KB)
+constexpr int kFewThreads = 256;    // workgroups for at most as many requests ...
+constexpr int kManyThreads = 1024;  // ... and for up to twice as many as these
+constexpr int kMostScanned = 2 * kManyThreads;
 constexpr int kTokensPerThread = 4;
-constexpr int kScanThreads = 1024;
 constexpr int64_t kLongest = 0x7fffffff;
 
 struct TableArgs {
@@ -33,6 +34,7 @@ struct TableArgs {
   int64_t width;
   int64_t table_stride;
   uint32_t block_size;
+  int32_t block_shift;  // log2 of it, or -1
   const int32_t* free_blocks;
   int64_t num_free;
   const int64_t* free_start;
@@ -48,86 +50,44 @@ struct TableArgs {
 };
 
 template <bool L64>
-__device__ __forceinline__ int64_t length_at(const void* p, int64_t i) {
+__device__ __forceinline__ uint32_t length_at(const void* p, int64_t i) {
   const int64_t v = L64 ? reinterpret_cast<const int64_t*>(p)[i]
                         : (int64_t) reinterpret_cast<const int32_t*>(p)[i];
-  return v < 0 ? 0 : (v > kLongest ? kLongest : v);
+  return (uint32_t)(v < 0 ? 0 : (v > kLongest ? kLongest : v));
 }
 
-// Exclusive prefix sum of one value per thread over a workgroup of THREADS; returns the total too.
-template <int THREADS>
-__device__ __forceinline__ int64_t workgroup_scan(int64_t v, int64_t& total, int64_t* s_wave) {
-  const int lane = threadIdx.x & 63;
-  const int wave = threadIdx.x >> 6;
-  int64_t inc = v;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t up = __shfl_up(inc, d, 64);
-    if (lane >= d) inc += up;
-  }
-  __syncthreads();  // s_wave may still be read from the scan before
-  if (lane == 63) s_wave[wave] = inc;
-  __syncthreads();
-  int64_t before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < THREADS / 64; ++w) {
-    if (w < wave) before += s_wave[w];
-    total += s_wave[w];
-  }
-  return before + inc - v;
+__device__ __forceinline__ uint32_t block_of(const TableArgs& a, uint32_t position) {
+  return a.block_shift >= 0 ? position >> a.block_shift : position / a.block_size;
 }
 
-__device__ __forceinline__ int64_t blocks_for(int64_t len, uint32_t bs, int64_t width) {
-  const uint32_t n = (uint32_t)len;  // both parts of a length are below 2^31
-  const int64_t b = n / bs + (n % bs != 0 ? 1 : 0);
-  return b < width ? b : width;
+// Blocks of the first `length` (below 2^32) tokens, as far as the table holds them.
+__device__ __forceinline__ uint32_t blocks_for(const TableArgs& a, uint32_t length) {
+  const uint32_t whole = block_of(a, length);
+  const uint32_t blocks = whole + (length - whole * a.block_size != 0 ? 1 : 0);
+  return blocks < (uint32_t)a.width ? blocks : (uint32_t)a.width;
 }
 
-// Blocks that a request with c tokens takes for n more.
-__device__ __forceinline__ int64_t blocks_taken(int64_t c, int64_t n, uint32_t bs, int64_t width) {
-  return blocks_for(c + n, bs, width) - blocks_for(c, bs, width);
+// Blocks that a request with c tokens takes for n more (c + n below 2^32).
+__device__ __forceinline__ uint32_t blocks_taken(const TableArgs& a, uint32_t c, uint32_t n) {
+  return blocks_for(a, c + n) - blocks_for(a, c);
 }
 
-// One workgroup: the prefix sums of all requests, each thread a contiguous span of them.
-// start(r, tokens before r) and taken(r, blocks before r) receive them; start(requests, ...) too.
-template <int THREADS, bool L64, typename Start, typename Taken>
-__device__ __forceinline__ void scan_requests(const TableArgs& a, int64_t* s_wave, Start start,
-                                              Taken taken, int64_t& all_taken) {
-  const int64_t per = (a.requests + THREADS - 1) / THREADS;
-  const int64_t r0 = threadIdx.x * per;
-  const int64_t r1 = r0 + per < a.requests ? r0 + per : a.requests;
-  int64_t sum = 0;
-  for (int64_t r = r0; r < r1; ++r) sum += length_at<L64>(a.fresh, r);
-  int64_t total;
-  int64_t at = workgroup_scan<THREADS>(sum, total, s_wave);
-  int64_t blocks = 0;
-  for (int64_t r = r0; r < r1; ++r) {
-    const int64_t n = length_at<L64>(a.fresh, r);
-    const int64_t b = at < a.tokens ? at : a.tokens;
-    const int64_t e = at + n < a.tokens ? at + n : a.tokens;
-    start(r, b, e);
-    blocks += blocks_taken(length_at<L64>(a.computed, r), e - b, a.block_size, a.width);
-    at += n;
-  }
-  int64_t before = workgroup_scan<THREADS>(blocks, all_taken, s_wave);
-  at = 0;
-  for (int64_t r = r0; r < r1; ++r) {
-    const int64_t t = taken(r, before);
-    before += t;
-  }
+// The sequence length of a request with c tokens computed and n new ones.
+__device__ __forceinline__ int32_t sequence_length(uint32_t c, uint32_t n) {
+  const uint32_t length = c + n;
+  return (int32_t)(length < (uint32_t)kLongest ? length : (uint32_t)kLongest);
 }
 
 // The outputs of token t of request r (its first token at `first`, `c` tokens computed before,
 // `before` blocks taken by the requests before it).
 __device__ __forceinline__ void write_token(const TableArgs& a, int64_t t, int64_t r, int64_t first,
-                                            int64_t c, int64_t before, int64_t free_start) {
-  const uint32_t p = (uint32_t)(c + (t - first));  // < 2^32: both are below 2^31
-  const uint32_t block = p / a.block_size;
+                                            uint32_t c, int64_t before, int64_t free_start) {
+  const uint32_t p = c + (uint32_t)(t - first);  // < 2^32: both are below 2^31
+  const uint32_t block = block_of(a, p);
   const uint32_t within = p - block * a.block_size;
   int64_t slot = -1;
-  if (block < a.width) {
-    const int64_t have = blocks_for(c, a.block_size, a.width);
+  if (block < (uint32_t)a.width) {
+    const uint32_t have = blocks_for(a, c);
     int32_t id;
     if (block < have) {
       id = a.tables[r * a.table_stride + block];
@@ -152,124 +112,177 @@ __device__ __forceinline__ void write_padding(const TableArgs& a, int64_t t) {
 // Last request whose first token is at or before t (starts[requests] is the number of tokens
 // held, and t < that).
 template <typename P>
-__device__ __forceinline__ int64_t find_request(P starts, int64_t requests, int64_t t) {
-  int64_t lo = 0, hi = requests;
+__device__ __forceinline__ int32_t find_request(P starts, int32_t requests, int32_t t) {
+  int32_t lo = 0, hi = requests;
   while (hi - lo > 1) {
-    const int64_t mid = (lo + hi) >> 1;
-    if ((int64_t)starts[mid] <= t) lo = mid; else hi = mid;
+    const int32_t mid = (int32_t)(((uint32_t)lo + (uint32_t)hi) >> 1);
+    if (starts[mid] <= t) lo = mid; else hi = mid;
   }
   return lo;
 }
 
-// The sequence length of a request with c tokens computed and n new ones.
-__device__ __forceinline__ int32_t sequence_length(int64_t c, int64_t n) {
-  return (int32_t)(c + n < kLongest ? c + n : kLongest);
-}
-
-template <bool L64>
-__global__ __launch_bounds__(kThreads) void tables_kernel(TableArgs a) {
-  __shared__ int32_t s_start[kOneLaunch + 1];
-  __shared__ int32_t s_computed[kOneLaunch];
-  __shared__ int64_t s_taken[kOneLaunch];
-  __shared__ int64_t s_wave[kThreads / 64];
+// One launch: every workgroup scans all requests (REQUESTS consecutive ones per thread), then
+// writes its tokens; the first one writes the requests' outputs too.
+template <int THREADS, int REQUESTS, bool L64>
+__global__ __launch_bounds__(THREADS) void tables_kernel(TableArgs a) {
+  constexpr int kMost = THREADS * REQUESTS;
+  constexpr int kWaves = THREADS / 64;
+  __shared__ int32_t s_start[kMost + 1];
+  __shared__ uint32_t s_computed[kMost];
+  __shared__ int64_t s_taken[kMost];
+  __shared__ uint64_t s_wave[kWaves];
   const int64_t free_start = a.free_start ? *a.free_start : 0;
-  int64_t all_taken;
-  if (a.requests == 0 && threadIdx.x == 0) s_start[0] = 0;
-  scan_requests<kThreads, L64>(
-      a, s_wave,
-      [&](int64_t r, int64_t b, int64_t e) {
-        s_start[r] = (int32_t)b;
-        s_start[r + 1] = (int32_t)e;  // the next request's own start: the same value
-        s_computed[r] = (int32_t)length_at<L64>(a.computed, r);
-      },
-      [&](int64_t r, int64_t before) {
-        s_taken[r] = before;
-        return blocks_taken(s_computed[r], s_start[r + 1] - s_start[r], a.block_size, a.width);
-      },
-      all_taken);
+  const int32_t requests = (int32_t)a.requests;
+  const int32_t r0 = REQUESTS * (int32_t)threadIdx.x;
+  uint32_t c[REQUESTS], n[REQUESTS];
+  uint64_t sum = 0, total;
+#pragma unroll
+  for (int j = 0; j < REQUESTS; ++j) {
+    c[j] = r0 + j < requests ? length_at<L64>(a.computed, r0 + j) : 0;
+    n[j] = r0 + j < requests ? length_at<L64>(a.fresh, r0 + j) : 0;
+    sum += n[j];
+  }
+  uint64_t at = workgroup_scan<kWaves, uint64_t>(sum, s_wave, total);
+  uint64_t taken = 0;
+#pragma unroll
+  for (int j = 0; j < REQUESTS; ++j) {
+    const uint64_t end = at + n[j];
+    const uint32_t b = at < (uint64_t)a.tokens ? (uint32_t)at : (uint32_t)a.tokens;
+    const uint32_t e = end < (uint64_t)a.tokens ? (uint32_t)end : (uint32_t)a.tokens;
+    at = end;
+    n[j] = e - b;  // the tokens that fit
+    taken += blocks_taken(a, c[j], n[j]);
+    if (r0 + j <= requests) s_start[r0 + j] = (int32_t)b;
+    if (r0 + j < requests) s_computed[r0 + j] = c[j];
+  }
+  if (requests == kMost && threadIdx.x == THREADS - 1)
+    s_start[kMost] = (int32_t)(total < (uint64_t)a.tokens ? total : (uint64_t)a.tokens);
+  uint64_t all_taken;
+  uint64_t before = workgroup_scan<kWaves, uint64_t>(taken, s_wave, all_taken);
+#pragma unroll
+  for (int j = 0; j < REQUESTS; ++j) {
+    if (r0 + j < requests) s_taken[r0 + j] = (int64_t)before;
+    before += blocks_taken(a, c[j], n[j]);
+  }
   __syncthreads();
-  const int64_t held = s_start[a.requests];
-  const int64_t t0 = (int64_t)blockIdx.x * (kThreads * kTokensPerThread) + threadIdx.x;
+  const int32_t held = s_start[requests];
+  const int64_t t0 = (int64_t)blockIdx.x * (THREADS * kTokensPerThread) + threadIdx.x;
 #pragma unroll
   for (int j = 0; j < kTokensPerThread; ++j) {
-    const int64_t t = t0 + j * kThreads;
+    const int64_t t = t0 + j * THREADS;
     if (t >= a.tokens) break;
     if (t >= held) {
       write_padding(a, t);
       continue;
     }
-    const int64_t r = find_request(s_start, a.requests, t);
+    const int32_t r = find_request(s_start, requests, (int32_t)t);
     write_token(a, t, r, s_start[r], s_computed[r], s_taken[r], free_start);
   }
   if (blockIdx.x == 0) {
-    for (int64_t r = threadIdx.x; r <= a.requests; r += kThreads) {
-      a.query_starts[r] = s_start[r];
-      if (r < a.requests)
-        a.seq_lens[r] = sequence_length(s_computed[r], s_start[r + 1] - s_start[r]);
+#pragma unroll
+    for (int j = 0; j < REQUESTS; ++j) {
+      const int32_t r = r0 + j;
+      if (r < requests) {
+        a.query_starts[r] = s_start[r];
+        a.seq_lens[r] = sequence_length(c[j], n[j]);
+      }
     }
     // (In place of free_start only where this is the only workgroup: every thread read it before
     // the scan's barriers.)
-    if (threadIdx.x == 0) *a.free_end = free_start + all_taken;
+    if (threadIdx.x == 0) {
+      a.query_starts[requests] = held;
+      *a.free_end = free_start + (int64_t)all_taken;
+    }
   }
 }
 
-// More requests than a workgroup scans on the side: the scan once, then the tokens.
+// More requests than a workgroup scans on the side: the scan once, each thread a contiguous span
+// of requests, then the tokens.
 template <bool L64>
-__global__ __launch_bounds__(kScanThreads) void scan_kernel(TableArgs a) {
-  __shared__ int64_t s_wave[kScanThreads / 64];
+__global__ __launch_bounds__(kManyThreads) void scan_kernel(TableArgs a) {
+  constexpr int kWaves = kManyThreads / 64;
+  __shared__ uint64_t s_wave[kWaves];
   const int64_t free_start = a.free_start ? *a.free_start : 0;
-  int64_t all_taken;
-  scan_requests<kScanThreads, L64>(
-      a, s_wave,
-      [&](int64_t r, int64_t b, int64_t e) {
-        a.query_starts[r] = (int32_t)b;
-        if (r == a.requests - 1) a.query_starts[a.requests] = (int32_t)e;
-        a.seq_lens[r] = sequence_length(length_at<L64>(a.computed, r), e - b);
-      },
-      [&](int64_t r, int64_t before) {
-        a.ws_taken[r] = before;
-        // (The starts written above, by this thread: they hold the tokens kept.)
-        const int64_t c = length_at<L64>(a.computed, r);
-        const int64_t b = a.query_starts[r];
-        const int64_t n = length_at<L64>(a.fresh, r);
-        return blocks_taken(c, b + n < a.tokens ? n : a.tokens - b, a.block_size, a.width);
-      },
-      all_taken);
-  if (a.requests == 0 && threadIdx.x == 0) a.query_starts[0] = 0;
+  const int64_t per = (a.requests + kManyThreads - 1) / kManyThreads;
+  const int64_t r0 = threadIdx.x * per;
+  const int64_t r1 = r0 + per < a.requests ? r0 + per : a.requests;
+  uint64_t sum = 0, total;
+  for (int64_t r = r0; r < r1; ++r) sum += length_at<L64>(a.fresh, r);
+  uint64_t at = workgroup_scan<kWaves, uint64_t>(sum, s_wave, total);
+  const uint64_t first = at;
+  const auto fitting = [&](int64_t r, uint32_t& start) {
+    const uint64_t end = at + length_at<L64>(a.fresh, r);
+    start = at < (uint64_t)a.tokens ? (uint32_t)at : (uint32_t)a.tokens;
+    at = end;
+    return (end < (uint64_t)a.tokens ? (uint32_t)end : (uint32_t)a.tokens) - start;
+  };
+  uint64_t taken = 0;
+  for (int64_t r = r0; r < r1; ++r) {
+    uint32_t start;
+    const uint32_t c = length_at<L64>(a.computed, r);
+    const uint32_t n = fitting(r, start);
+    a.query_starts[r] = (int32_t)start;
+    a.seq_lens[r] = sequence_length(c, n);
+    taken += blocks_taken(a, c, n);
+  }
+  uint64_t all_taken;
+  uint64_t before = workgroup_scan<kWaves, uint64_t>(taken, s_wave, all_taken);
+  at = first;
+  for (int64_t r = r0; r < r1; ++r) {
+    uint32_t start;
+    a.ws_taken[r] = (int64_t)before;
+    const uint32_t n = fitting(r, start);
+    before += blocks_taken(a, length_at<L64>(a.computed, r), n);
+  }
   if (threadIdx.x == 0) {
+    a.query_starts[a.requests] = (int32_t)(total < (uint64_t)a.tokens ? total : (uint64_t)a.tokens);
     *a.ws_free = free_start;
-    *a.free_end = free_start + all_taken;
+    *a.free_end = free_start + (int64_t)all_taken;
   }
 }
 
 template <bool L64>
-__global__ __launch_bounds__(kThreads) void tokens_kernel(TableArgs a) {
-  const int64_t held = a.query_starts[a.requests];
+__global__ __launch_bounds__(kFewThreads) void tokens_kernel(TableArgs a) {
+  const int32_t held = a.query_starts[a.requests];
   const int64_t free_start = *a.ws_free;
-  const int64_t t0 = (int64_t)blockIdx.x * (kThreads * kTokensPerThread) + threadIdx.x;
+  const int64_t t0 = (int64_t)blockIdx.x * (kFewThreads * kTokensPerThread) + threadIdx.x;
 #pragma unroll
   for (int j = 0; j < kTokensPerThread; ++j) {
-    const int64_t t = t0 + j * kThreads;
+    const int64_t t = t0 + j * kFewThreads;
     if (t >= a.tokens) break;
     if (t >= held) {
       write_padding(a, t);
       continue;
     }
-    const int64_t r = find_request(a.query_starts, a.requests, t);
+    const int32_t r = find_request(a.query_starts, (int32_t)a.requests, (int32_t)t);
     write_token(a, t, r, a.query_starts[r], length_at<L64>(a.computed, r), a.ws_taken[r], free_start);
   }
 }
 
+uint32_t grid_for(int64_t tokens, int threads) {
+  const int64_t per_wg = threads * kTokensPerThread;
+  return (uint32_t)((tokens + per_wg - 1) / per_wg);
+}
+
+template <int THREADS, int REQUESTS, bool L64>
+void launch_one(const TableArgs& a, hipStream_t s) {
+  const uint32_t grid = grid_for(a.tokens, THREADS);
+  hipLaunchKernelGGL((tables_kernel<THREADS, REQUESTS, L64>), dim3(grid > 0 ? grid : 1),
+                     dim3(THREADS), 0, s, a);
+}
+
 template <bool L64>
-void launch(const TableArgs& a, bool one_launch, hipStream_t s) {
-  const int64_t per_wg = kThreads * kTokensPerThread;
-  const uint32_t grid = (uint32_t)((a.tokens + per_wg - 1) / per_wg);
-  if (one_launch) {
-    hipLaunchKernelGGL(tables_kernel<L64>, dim3(grid > 0 ? grid : 1), dim3(kThreads), 0, s, a);
-    return;
-  }
-  hipLaunchKernelGGL(scan_kernel<L64>, dim3(1), dim3(kScanThreads), 0, s, a);
-  if (grid > 0) hipLaunchKernelGGL(tokens_kernel<L64>, dim3(grid), dim3(kThreads), 0, s, a);
+void launch(const TableArgs& a, bool in_place, hipStream_t s) {
+  // free_end in place of free_start: one workgroup alone may read and write it in one launch.
+  if (a.requests <= kFewThreads && !(in_place && grid_for(a.tokens, kFewThreads) > 1))
+    return launch_one<kFewThreads, 1, L64>(a, s);
+  if (a.requests <= kManyThreads && !(in_place && grid_for(a.tokens, kManyThreads) > 1))
+    return launch_one<kManyThreads, 1, L64>(a, s);
+  if (a.requests <= kMostScanned && !(in_place && grid_for(a.tokens, kManyThreads) > 1))
+    return launch_one<kManyThreads, 2, L64>(a, s);
+  hipLaunchKernelGGL(scan_kernel<L64>, dim3(1), dim3(kManyThreads), 0, s, a);
+  const uint32_t grid = grid_for(a.tokens, kFewThreads);
+  if (grid > 0) hipLaunchKernelGGL(tokens_kernel<L64>, dim3(grid), dim3(kFewThreads), 0, s, a);
 }
 
 }  // namespace
@@ -278,7 +291,7 @@ void launch(const TableArgs& a, bool one_launch, hipStream_t s) {
 using namespace int8kv_serving;
 
 extern "C" size_t int8kv_batch_tables_workspace_bytes(int64_t requests) {
-  if (requests < 0 || requests > 0x7fffffff) return 0;
+  if (requests < 0 || requests > 0x7ffffffe) return 0;
   return 16 + 8 * (size_t)requests;
 }
 
@@ -313,6 +326,7 @@ extern "C" int int8kv_batch_tables(const void* computed_lens, const void* new_le
   a.width = table_width;
   a.table_stride = table_row_stride;
   a.block_size = (uint32_t)block_size;
+  a.block_shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctz((unsigned)block_size) : -1;
   a.free_blocks = free_blocks;
   a.num_free = num_free;
   a.free_start = free_start;
@@ -325,13 +339,10 @@ extern "C" int int8kv_batch_tables(const void* computed_lens, const void* new_le
   a.free_end = free_end;
   a.ws_free = static_cast<int64_t*>(workspace);
   a.ws_taken = a.ws_free + 2;
-  // free_end in place of free_start: one workgroup alone may read and write it in one launch.
-  const bool in_place = free_start == free_end && num_tokens > kThreads * kTokensPerThread;
-  const bool one_launch = requests <= kOneLaunch && !in_place;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (lens_dtype == INT8KV_I64)
-    launch<true>(a, one_launch, s);
+    launch<true>(a, free_start == free_end, s);
   else
-    launch<false>(a, one_launch, s);
+    launch<false>(a, free_start == free_end, s);
   return (int)hipGetLastError();
 }

@@ -17,6 +17,7 @@
 
 #include "int8kv_common.h"
 #include "serving_ops.h"
+#include "wave_scan.h"
 
 namespace int8kv_serving {
 namespace {
@@ -207,36 +208,10 @@ struct FastWeights {
 __device__ __forceinline__ void lds_barrier() {
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
-// A lane's value moved along the wave without LDS (DPP): CTRL row_shr 1, 2, 4, 8 within 16 lanes,
-// row_bcast 15 and 31 across them.  Lanes without a source keep `old`.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t dpp(uint32_t old, uint32_t v) {
-  return (uint32_t)__builtin_amdgcn_update_dpp((int)old, (int)v, CTRL, ROWS, 0xf, false);
-}
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t dpp_add(uint32_t v) {
-  return v + dpp<CTRL, ROWS>(0u, v);
-}
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint64_t dpp_add(uint64_t v) {
-  const uint32_t lo = dpp<CTRL, ROWS>(0u, (uint32_t)v);
-  const uint32_t hi = dpp<CTRL, ROWS>(0u, (uint32_t)(v >> 32));
-  return v + (((uint64_t)hi << 32) | lo);
-}
 template <int CTRL, int ROWS>
 __device__ __forceinline__ float dpp_max(float v) {
   const uint32_t b = __float_as_uint(v);
   return fmaxf(v, __uint_as_float(dpp<CTRL, ROWS>(b, b)));
-}
-// Inclusive prefix sum over the wave.
-template <typename T>
-__device__ __forceinline__ T wave_scan(T v) {
-  v = dpp_add<0x111, 0xf>(v);
-  v = dpp_add<0x112, 0xf>(v);
-  v = dpp_add<0x114, 0xf>(v);
-  v = dpp_add<0x118, 0xf>(v);
-  v = dpp_add<0x142, 0xa>(v);
-  return dpp_add<0x143, 0xc>(v);
 }
 // The largest (or smallest) of the lanes' values, in lane 63.
 template <bool LARGEST>
@@ -249,13 +224,6 @@ __device__ __forceinline__ uint32_t wave_extreme(uint32_t v) {
   v = pick(v, dpp<0x142, 0xa>(v, v));
   return pick(v, dpp<0x143, 0xc>(v, v));
 }
-__device__ __forceinline__ uint32_t last_lane(uint32_t v, int lane = 63) {
-  return (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
-}
-__device__ __forceinline__ uint64_t last_lane(uint64_t v, int lane = 63) {
-  return ((uint64_t)last_lane((uint32_t)(v >> 32), lane) << 32) | last_lane((uint32_t)v, lane);
-}
-__device__ __forceinline__ uint64_t wave_sum(uint64_t v) { return last_lane(wave_scan(v)); }
 // Running maximum: lane 15 of each 16, then lanes 31 and 63 hold their 32 lanes', then lane 63 all.
 __device__ __forceinline__ float max_to_31(float m) {
   m = dpp_max<0x111, 0xf>(m);
@@ -268,26 +236,6 @@ __device__ __forceinline__ float max_to_63(float m) { return dpp_max<0x143, 0xc>
 __device__ __forceinline__ float wave_max(float m) {
   return __uint_as_float(last_lane(__float_as_uint(max_to_63(max_to_31(m)))));
 }
-// Exclusive prefix sum over the workgroup; s_wave: kWaves values.
-template <typename T>
-__device__ __forceinline__ T workgroup_scan(T v, T* s_wave, T& total) {
-  static_assert(kWaves <= 16, "the waves' sums are scanned by 16 lanes");
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const T inc = wave_scan(v);
-  __syncthreads();
-  if (lane == 63) s_wave[wave] = inc;
-  __syncthreads();
-  T w = s_wave[lane & (kWaves - 1)];
-  w = dpp_add<0x111, 0xf>(w);
-  w = dpp_add<0x112, 0xf>(w);
-  w = dpp_add<0x114, 0xf>(w);
-  w = dpp_add<0x118, 0xf>(w);
-  total = last_lane(w, kWaves - 1);
-  const T before = wave > 0 ? last_lane(w, wave - 1) : 0;
-  return before + inc - v;
-}
-
 // --------------------------------------------------------------------------- row parameters
 struct Params {
   double u;
@@ -484,7 +432,7 @@ __device__ __forceinline__ uint64_t scan_chunks(const SampleArgs& a, int64_t r, 
       mass = (uint64_t)rint((double)own * factor);
     }
   }
-  return workgroup_scan<uint64_t>(mass, s_wave, total);
+  return workgroup_scan<kWaves, uint64_t>(mass, s_wave, total);
 }
 
 // Tiles of a row: 1, 2, 4 ... pieces, at most kMaxTiles of them, each a power of two of slots.
@@ -705,8 +653,8 @@ __device__ bool select_key(const Row<DT>& row, const Weights& w, uint64_t want, 
     const uint64_t m0 = s.mass[b0], m1 = s.mass[b0 - 1];
     uint32_t ctot;
     uint64_t mtot;
-    const uint32_t cb = workgroup_scan<uint32_t>(c0 + c1, s.wave32, ctot);
-    const uint64_t mb = workgroup_scan<uint64_t>(m0 + m1, s.wave64, mtot);
+    const uint32_t cb = workgroup_scan<kWaves, uint32_t>(c0 + c1, s.wave32, ctot);
+    const uint64_t mb = workgroup_scan<kWaves, uint64_t>(m0 + m1, s.wave64, mtot);
     const uint64_t left = want - (BY_MASS ? mass_above : (uint64_t)count_above);
     const uint64_t x0 = BY_MASS ? mb : (uint64_t)cb;
     const uint64_t x1 = x0 + (BY_MASS ? m0 : (uint64_t)c0);
@@ -757,7 +705,7 @@ __device__ Cut find_cut(const Row<DT>& row, const Weights& w, const Params& q, G
 #pragma unroll
         for (int j = 0; j < Row<DT>::kE; ++j) sum += w(v[j]);
       }
-      workgroup_scan<uint64_t>(sum, s.wave64, kept);
+      workgroup_scan<kWaves, uint64_t>(sum, s.wave64, kept);
     }
     // Tokens whose preceding mass is below p S(n_k): up to the one that reaches it.
     uint64_t want = (uint64_t)ceil(q.p * (double)kept);
@@ -902,7 +850,7 @@ __device__ __forceinline__ uint64_t cut_list(const Weights& w, const Params& q, 
   }
   __syncthreads();
   uint64_t total;
-  const uint64_t before = workgroup_scan<uint64_t>(sum, s.wave64, total);
+  const uint64_t before = workgroup_scan<kWaves, uint64_t>(sum, s.wave64, total);
   // S(n_k): of the first k, or everything.
   const bool top_k = q.k > 0 && q.k < n;
   int32_t last = top_k ? q.k - 1 : n - 1;
@@ -1010,8 +958,8 @@ __device__ __forceinline__ bool cut_by_bins(const Weights& w, const Params& q, c
   const uint64_t m0 = s.list.bin_mass[2 * t], m1 = s.list.bin_mass[2 * t + 1];
   uint32_t count_all;
   uint64_t mass_all = 0, mb = 0;
-  const uint32_t cb = workgroup_scan<uint32_t>(c0 + c1, s.wave32, count_all);
-  if (q.p < 1.0) mb = workgroup_scan<uint64_t>(m0 + m1, s.wave64, mass_all);
+  const uint32_t cb = workgroup_scan<kWaves, uint32_t>(c0 + c1, s.wave32, count_all);
+  if (q.p < 1.0) mb = workgroup_scan<kWaves, uint64_t>(m0 + m1, s.wave64, mass_all);
   const bool top_k = q.k > 0 && q.k < n;
   uint64_t kept = mass_all;
   last = 0;  // (everything)
@@ -1032,7 +980,7 @@ __device__ __forceinline__ bool cut_by_bins(const Weights& w, const Params& q, c
     if (t == left - 1) s.value64[1] = place;
     uint64_t sum = 0;
     if (q.p < 1.0)
-      workgroup_scan<uint64_t>(t < left ? w(value_of(place_key(place))) : 0, s.wave64, sum);
+      workgroup_scan<kWaves, uint64_t>(t < left ? w(value_of(place_key(place))) : 0, s.wave64, sum);
     else
       __syncthreads();
     kept += sum;
@@ -1057,7 +1005,7 @@ __device__ __forceinline__ bool cut_by_bins(const Weights& w, const Params& q, c
     if (count > kRanked) return false;
     const uint64_t mass = t < count ? w(value_of(place_key(place))) : 0;
     uint64_t sum;
-    const uint64_t at = before_bin + workgroup_scan<uint64_t>(mass, s.wave64, sum);
+    const uint64_t at = before_bin + workgroup_scan<kWaves, uint64_t>(mass, s.wave64, sum);
     if (at < want && want <= at + mass) s.value64[1] = place;  // one thread
     __syncthreads();
     last = s.value64[1];
@@ -1160,7 +1108,7 @@ __device__ __forceinline__ void finish_plain(const SampleArgs& a, const Row<DT>&
 #pragma unroll
   for (int j = 0; j < kE; ++j) sum += x[j];
   uint64_t all;
-  uint64_t at = workgroup_scan<uint64_t>(sum, s.wave64, all);
+  uint64_t at = workgroup_scan<kWaves, uint64_t>(sum, s.wave64, all);
   if (left >= all) left = all - 1;  // (a sum of several weights may round otherwise than each)
   if (at <= left && left < at + sum) {  // one thread
     int32_t pick = 0;
@@ -1189,7 +1137,7 @@ __device__ __forceinline__ void finish_tiles(const SampleArgs& a, const Row<DT>&
     s.value32[0] = 0;
   }
   uint64_t total;
-  const uint64_t before = workgroup_scan<uint64_t>(mass, s.wave64, total);
+  const uint64_t before = workgroup_scan<kWaves, uint64_t>(mass, s.wave64, total);
   const uint64_t target = scaled(q.u, total);
   if (before <= target && target < before + mass) {  // one thread
     s.value64[0] = target - before;
@@ -1249,7 +1197,7 @@ __device__ __attribute__((noinline)) void finish_general(const SampleArgs& a, in
   const int t = threadIdx.x;
   const uint32_t n = t < tiles ? s.tile_ties[t] : 0;
   uint32_t all_ties;
-  const uint32_t before = workgroup_scan<uint32_t>(n, s.wave32, all_ties);
+  const uint32_t before = workgroup_scan<kWaves, uint32_t>(n, s.wave32, all_ties);
   const uint32_t left = cut.ties > before ? cut.ties - before : 0;
   if (t == 0) s.value32[2] = -1;
   __syncthreads();
@@ -1292,7 +1240,7 @@ __device__ __forceinline__ int32_t find_bin(const T* bins, T want, T* s_wave, Ro
     sum += x[j];
   }
   if (threadIdx.x == 0) s.value32[6] = kBins;
-  T at = workgroup_scan<T>(sum, s_wave, total);
+  T at = workgroup_scan<kWaves, T>(sum, s_wave, total);
   if (at < want && want <= at + sum) {  // one thread
     int32_t bin = b0;
 #pragma unroll
