@@ -529,6 +529,77 @@ __device__ __forceinline__ void read_tiles(const Row<DT>& row, const Tiles<DT>& 
   }
 }
 
+// The same for tokens far apart (a few per tile): slots that hold one are queued whole and looked
+// through afterwards, so that reading costs a maximum and a comparison per slot.
+constexpr int kSlotQueue = 1024;
+struct SlotQueue {
+  u32x4 raw[kSlotQueue];
+  int32_t slot[kSlotQueue];
+  int32_t length;
+};
+template <int DT, typename Token>
+__device__ __forceinline__ void read_tiles_sparse(const Row<DT>& row, const Tiles<DT>& tiles,
+                                                  const int32_t* visit, int32_t visits, float from,
+                                                  SlotQueue& queue, Token token) {
+  constexpr int kE = Row<DT>::kE;
+  constexpr int kTogether = 4;
+  const int32_t items = visits << tiles.shift;
+  const float least = fmaxf(from, -3.4028235e38f);
+  const auto slot_of = [&](int32_t i) {
+    return i < items ? (visit[i >> tiles.shift] << tiles.shift) + (i & (tiles.slots - 1)) : -1;
+  };
+  const auto look = [&](int32_t slot, u32x4 raw) {
+    float v[kE];
+    row.template values<false>(slot, raw, v);
+#pragma unroll
+    for (int j = 0; j < kE; ++j)
+      if (v[j] >= least) token(v[j], row.first(slot) + j);
+  };
+  u32x4 raw[kTogether];
+  int32_t slot[kTogether];
+  const auto request = [&](int32_t i0) {
+#pragma unroll
+    for (int u = 0; u < kTogether; ++u) {
+      slot[u] = slot_of(i0 + u * kThreads + (int32_t)threadIdx.x);
+      raw[u] = row.request(slot[u]);
+    }
+  };
+  request(0);
+  for (int32_t i0 = 0; i0 < items; i0 += kTogether * kThreads) {
+    u32x4 now[kTogether];
+    int32_t at[kTogether];
+#pragma unroll
+    for (int u = 0; u < kTogether; ++u) {
+      now[u] = raw[u];
+      at[u] = slot[u];
+    }
+    request(i0 + kTogether * kThreads);
+#pragma unroll
+    for (int u = 0; u < kTogether; ++u) {
+      if (i0 + u * kThreads >= items) break;  // (uniform)
+      if (at[u] < 0) continue;
+      float v[kE];
+      row.template values<false>(at[u], now[u], v);
+      float m = v[0];
+#pragma unroll
+      for (int j = 1; j < kE; ++j) m = fmaxf(m, v[j]);
+      if (m >= least) {
+        const int32_t place = atomicAdd(&queue.length, 1);
+        if (place < kSlotQueue) {
+          queue.raw[place] = now[u];
+          queue.slot[place] = at[u];
+        } else {
+          look(at[u], now[u]);
+        }
+      }
+    }
+  }
+  __syncthreads();
+  const int32_t n = queue.length < kSlotQueue ? queue.length : kSlotQueue;
+  for (int32_t i = threadIdx.x; i < n; i += kThreads) look(queue.slot[i], queue.raw[i]);
+  __syncthreads();
+}
+
 // ------------------------------------------------------------------------ histogram pass
 // One part of one row with a nucleus cut alone: the weights of its tokens per bin, added to the
 // row's (integers: in any order).  Tokens with w < (1 - p) Z / vocab cannot be kept (they and all
@@ -738,7 +809,7 @@ struct RowShared {
       uint32_t bin_count[kBins];
     } list;
   };
-  Queue queue;
+  SlotQueue queue;
   uint64_t tile_mass[kMaxTiles];
   uint32_t tile_ties[kMaxTiles];
   int32_t visit[kMaxTiles];
@@ -812,6 +883,7 @@ __device__ __forceinline__ uint64_t rank_places(int32_t n, uint64_t* s) {
   if (e < n) {
     const uint64_t mine = s[e];
     int32_t above = 0;
+#pragma unroll 8
     for (int32_t j = j0; j < j1; ++j) above += s[j] > mine ? 1 : 0;
     if (above) atomicAdd(&rank[e], above);
   }
@@ -872,13 +944,13 @@ __device__ __forceinline__ uint64_t cut_list(const Weights& w, const Params& q, 
     uint64_t want = (uint64_t)ceil(q.p * (double)kept);
     want = want < 1 ? 1 : want;
     at = cut.before + before;
-    int32_t mine = -1;
 #pragma unroll
     for (int e = 0; e < P; ++e) {
-      if (t * P + e < n && at < want) mine = t * P + e;
+      const bool first = at < want;
       at += weight[e];
+      // (One of them: the token that reaches `want`, or the list's last.)
+      if (first && (at >= want || t * P + e == n - 1) && t * P + e < n) s.value32[0] = t * P + e;
     }
-    if (mine >= 0) atomicMax(&s.value32[0], mine);
     __syncthreads();
     last = s.value32[0] < last ? s.value32[0] : last;
   }
@@ -1152,6 +1224,29 @@ __device__ __forceinline__ void finish_tiles(const SampleArgs& a, const Row<DT>&
   }
 }
 
+// Rows whose list is short and holds every kept token: the list in index order.
+__device__ __forceinline__ void finish_list(const SampleArgs& a, int64_t r, const Params& q,
+                                            const Weights& w, uint64_t least, int32_t n,
+                                            uint64_t last_place, RowShared& s) {
+  const int t = threadIdx.x;
+  // By falling ~index, each with its key.
+  uint64_t* by_index = reinterpret_cast<uint64_t*>(&s.queue);
+  if (t < n) by_index[t] = (s.list.place[t] << 32) | (s.list.place[t] >> 32);
+  if (t == 0) {
+    s.value64[0] = 0;
+    s.value32[0] = 0;
+  }
+  __syncthreads();
+  const uint64_t mine = rank_places(n, by_index);
+  const uint64_t place = (mine << 32) | (mine >> 32);
+  uint64_t mass = t < n && place >= last_place ? w(value_of(place_key(place))) : 0;
+  mass = mass >= least ? mass : 0;
+  uint64_t total;
+  const uint64_t before = workgroup_scan<kWaves, uint64_t>(mass, s.wave64, total);
+  const uint64_t target = scaled(q.u, total);
+  if (before <= target && target < before + mass) a.out[r] = place_index(place);  // one thread
+}
+
 // The general path: cut by digits, then the kept weight of every tile, ties counted by index.
 // (Not inlined, and given a copy of the arguments: the row kernel keeps its registers.)
 template <int DT>
@@ -1226,10 +1321,10 @@ __device__ __attribute__((noinline)) void finish_general(const SampleArgs& a, in
   });
 }
 
-// The bin in which the cumulative sum of s.list.bin_mass (or bin_count) reaches `want`, and what
-// comes before that bin; kBins if the whole does not reach it.
-template <typename T>
-__device__ __forceinline__ int32_t find_bin(const T* bins, T want, T* s_wave, RowShared& s, T& before,
+// The bin in which the cumulative sum of `bins` reaches `want`, and what comes before that bin;
+// kBins if the whole does not reach it.
+template <typename T, typename Shared>
+__device__ __forceinline__ int32_t find_bin(const T* bins, T want, T* s_wave, Shared& s, T& before,
                                             T& total) {
   const int32_t b0 = (int32_t)threadIdx.x * kThreadBins;
   T x[kThreadBins];
@@ -1261,13 +1356,15 @@ __device__ __forceinline__ int32_t find_bin(const T* bins, T want, T* s_wave, Ro
   return bin;
 }
 
-// The bin in which a nucleus cut alone falls (histogram in s.list.bin_mass, `total` the row's mass).
-__device__ __forceinline__ int32_t nucleus_bin(const Params& q, uint64_t total, RowShared& s,
+// The bin in which a nucleus cut alone falls (`total`: the row's mass).
+template <typename Shared>
+__device__ __forceinline__ int32_t nucleus_bin(const Params& q, uint64_t total,
+                                               const uint64_t* bin_mass, Shared& s,
                                                uint64_t& before, uint64_t& binned) {
   const uint64_t want = (uint64_t)ceil(q.p * (double)total);
-  int32_t bin = find_bin<uint64_t>(s.list.bin_mass, want < 1 ? 1 : want, s.wave64, s, before, binned);
+  int32_t bin = find_bin<uint64_t>(bin_mass, want < 1 ? 1 : want, s.wave64, s, before, binned);
   // (Roundings: the tokens left out weigh less than (1 - p) Z, but p Z may be all but Z.)
-  if (bin == kBins) bin = find_bin<uint64_t>(s.list.bin_mass, binned, s.wave64, s, before, binned);
+  if (bin == kBins) bin = find_bin<uint64_t>(bin_mass, binned, s.wave64, s, before, binned);
   return bin;
 }
 
@@ -1279,33 +1376,26 @@ __device__ __forceinline__ float bin_from(int32_t bin, float top) {
   return (float)((double)top - (double)d) - fabsf(top) * 0x1p-20f;
 }
 
-// Puts the tokens down to bin `last` where they belong: those of bins from `first` on into
-// s.list.place, the weights of those before it to s.tile_mass (tile `base` first), `least` and
-// more.  s.visit, s.visits, s.length and s.queue.length are set.
-template <int DT>
-__device__ __forceinline__ void gather(const Row<DT>& row, const Tiles<DT>& tiles, const Weights& w,
-                                       int32_t first, int32_t last, uint64_t least, int32_t base,
-                                       RowShared& s) {
-  const float top = w.topf;
-  read_tiles(row, tiles, s.visit, s.visits, bin_from(last, top), s.queue, [&](float v, int32_t index) {
-    const int32_t b = bin_of(v, top);
-    if (b < first) {
-      const uint64_t x = w(v);
-      if (x >= least && x > 0)
-        atomicAdd(reinterpret_cast<unsigned long long*>(&s.tile_mass[tiles.of(row, index) - base]),
-                  (unsigned long long)x);
-    } else if (b <= last) {
-      const int32_t at = atomicAdd(&s.length, 1);
-      if (at < kList) s.list.place[at] = place_of(key_of(v), index);
-    }
-  });
-}
+struct GatherShared {
+  union {
+    uint64_t bin_mass[kBins];
+    Queue queue;  // (once the bin is found)
+  };
+  uint64_t place[kList];
+  uint64_t tile_mass[kMaxTiles];
+  int32_t visit[kMaxTiles];
+  uint64_t wave64[kWaves];
+  float wave_max[kWaves];
+  uint64_t value64[1];
+  int32_t value32[7];
+  int32_t visits, length;
+};
 
 // One part of the tiles of a row with a nucleus cut alone, its histogram finished: the tokens of
 // the bin where the cut falls, and the mass of those before it per tile.
 template <int DT>
 __global__ __launch_bounds__(kThreads) void gather_kernel(SampleArgs a) {
-  __shared__ RowShared s;
+  __shared__ GatherShared s;
   const int64_t r = blockIdx.x / a.parts;
   const int32_t part = (int32_t)(blockIdx.x - r * a.parts);
   const int t = threadIdx.x;
@@ -1316,23 +1406,36 @@ __global__ __launch_bounds__(kThreads) void gather_kernel(SampleArgs a) {
   const int32_t tile0 = part * per;
   const int32_t tile1 = tile0 + per < tiles.count ? tile0 + per : tiles.count;
   if (tile0 >= tile1) return;
-  for (int32_t b = t; b < kBins; b += kThreads) s.list.bin_mass[b] = a.bin_mass[r * kBins + b];
+  for (int32_t b = t; b < kBins; b += kThreads) s.bin_mass[b] = a.bin_mass[r * kBins + b];
   const float tile_max = t < tile1 - tile0 ? tiles.max_of(a, r, tile0 + t) : -INFINITY;
-  if (t == 0) s.visits = s.length = s.queue.length = 0;
+  if (t == 0) s.visits = s.length = 0;
   s.tile_mass[t] = 0;
   const float top = row_max(a, r, s.wave_max);  // (with a barrier)
   if (top == -INFINITY) return;
   const Row<DT> row(a, r);
   const Weights w{0x1.71547652b82fep+0 / (double)q.t, (double)top, top, a.frac};
+  const uint64_t least = least_weight(q.m, a.frac);
   float chunk_top;
   uint64_t own, mass, total, before, binned;
   double factor;
   scan_chunks(a, r, q, top, s.wave64, chunk_top, own, mass, factor, total);
-  const int32_t bin = nucleus_bin(q, total, s, before, binned);
-  if (tile_max >= bin_from(bin, top) && tile_max > -INFINITY)
-    s.visit[atomicAdd(&s.visits, 1)] = tile0 + t;
+  const int32_t bin = nucleus_bin(q, total, s.bin_mass, s, before, binned);
+  const float from = bin_from(bin, top);
+  if (t == 0) s.queue.length = 0;
+  if (tile_max >= from && tile_max > -INFINITY) s.visit[atomicAdd(&s.visits, 1)] = tile0 + t;
   __syncthreads();
-  gather(row, tiles, w, bin, bin, least_weight(q.m, a.frac), tile0, s);
+  read_tiles(row, tiles, s.visit, s.visits, from, s.queue, [&](float v, int32_t index) {
+    const int32_t b = bin_of(v, top);
+    if (b < bin) {
+      const uint64_t x = w(v);
+      if (x >= least && x > 0)
+        atomicAdd(reinterpret_cast<unsigned long long*>(&s.tile_mass[tiles.of(row, index) - tile0]),
+                  (unsigned long long)x);
+    } else if (b == bin) {
+      const int32_t at = atomicAdd(&s.length, 1);
+      if (at < kList) s.place[at] = place_of(key_of(v), index);
+    }
+  });
   __syncthreads();
   if (t < tile1 - tile0) a.tile_mass[r * kMaxTiles + tile0 + t] = s.tile_mass[t];
   const int32_t n = s.length;
@@ -1340,7 +1443,7 @@ __global__ __launch_bounds__(kThreads) void gather_kernel(SampleArgs a) {
   __syncthreads();
   const int32_t at = s.value32[6];
   for (int32_t i = t; i < n && i < kList && at + i < kList; i += kThreads)
-    a.list[r * kList + at + i] = s.list.place[i];
+    a.list[r * kList + at + i] = s.place[i];
 }
 
 // One row.  Rows without a filter need the chunks' masses only.  Otherwise the cut lies in a list
@@ -1406,7 +1509,7 @@ __global__ __launch_bounds__(kThreads) void row_kernel(SampleArgs a) {
     uint64_t own, mass, total, binned;
     double factor;
     scan_chunks(a, r, q, top, s.wave64, chunk_top, own, mass, factor, total);
-    nucleus_bin(q, total, s, cut.before, binned);
+    nucleus_bin(q, total, s.list.bin_mass, s, cut.before, binned);
     cut.all_mass = total < binned ? binned : total;
     const int32_t n = s.length < kList ? s.length : kList;
     for (int32_t i = t; i < n; i += kThreads) s.list.place[i] = a.list[r * kList + i];
@@ -1435,9 +1538,20 @@ __global__ __launch_bounds__(kThreads) void row_kernel(SampleArgs a) {
     if (confirmed && tile_max >= bin_from(last, top) && tile_max > -INFINITY)
       s.visit[atomicAdd(&s.visits, 1)] = t;
     __syncthreads();
-    // (min-p alone lists nothing: everything goes to the tiles.)
-    gather(row, tiles, w, filter ? 0 : kBins, last, least, 0, s);
-    __syncthreads();
+    // (min-p alone lists nothing: its tokens' weights go to their tiles.)
+    read_tiles_sparse(row, tiles, s.visit, s.visits, bin_from(last, top), s.queue,
+                      [&](float v, int32_t index) {
+      if (filter) {
+        if (bin_of(v, top) > last) return;
+        const int32_t at = atomicAdd(&s.length, 1);
+        if (at < kList) s.list.place[at] = place_of(key_of(v), index);
+      } else {
+        const uint64_t x = w(v);
+        if (x >= least && x > 0)
+          atomicAdd(reinterpret_cast<unsigned long long*>(&s.tile_mass[tiles.of(row, index)]),
+                    (unsigned long long)x);
+      }
+    });
     // The list holds the first k tokens, or every live one.
     confirmed = confirmed && (last == kBins - 1 || !filter || s.length >= q.k);
   }
@@ -1451,6 +1565,10 @@ __global__ __launch_bounds__(kThreads) void row_kernel(SampleArgs a) {
       return;
     }
     last_place = cut_list_any(w, q, cut, n, s);
+    if (!counted && n <= kRanked) {
+      finish_list(a, r, q, w, least, n, last_place, s);
+      return;
+    }
     for (int32_t i = t; i < n; i += kThreads) {
       const uint64_t p = s.list.place[i];
       const uint64_t x = w(value_of(place_key(p)));
@@ -1570,11 +1688,14 @@ extern "C" int int8kv_sample_rows(const void* logits, int logits_dtype, int64_t 
   a.run_chunks = (int32_t)(per_unit < 1 ? 1 : (per_unit < 8 ? per_unit : 8));
   a.runs = (a.chunks + a.run_chunks - 1) / a.run_chunks;
   // The histogram pass and the gathering behind it run where some row may have a nucleus cut alone
-  // and more tokens than its list holds: about one workgroup per compute unit.
+  // and more tokens than its list holds.  A compute unit takes one of their workgroups; parts for
+  // twice the units, since rows with other settings leave at once (61 rows of mixed settings: 13 us
+  // each with 8 parts, 18 with 4), unless two rows out of three would wait for a second turn (200
+  // rows, all with a nucleus cut: 23 and 19 us with 1 part, 25 and 23 with 2).
   a.parts = 0;
   if (top_p && a.pieces > kList / kPieceElements) {
     const int64_t most = (vocab + 4 * kThreads - 1) / (4 * kThreads);
-    const int64_t want = 256 / rows < 1 ? 1 : 256 / rows;
+    const int64_t want = rows <= 128 ? 512 / rows : (256 / rows < 1 ? 1 : 256 / rows);
     a.parts = (int32_t)(want < most ? want : most);
   }
   if (logits_dtype == INT8KV_F32)
