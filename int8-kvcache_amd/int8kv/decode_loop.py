@@ -11,6 +11,10 @@ vllm_int8/vllm_int8_attention_patch.py in "int8_only" mode):
   scatter) and attends with ``int8kv_paged_decode`` over the INT8 or the BF16 cache;
 * a decode step is one HIP graph: the sequence state (next token, position, length, slot) lives
   in device buffers updated inside the graph, so a replay is one step with no host work.
+* on request (``DecodeLoop(..., sampling=, adapters=, on_demand=)``) the tokens are sampled
+  (``sample_tokens``) instead of taken greedily, every sequence has its own low-rank adapter on the
+  projections (``lora_plan`` / ``lora_add``), and its blocks come from a free list when its tokens
+  need them (``build_batch_tables``), all inside the graph.
 
 Model (Qwen2 architecture, random weights, no checkpoint): token embedding; per layer RMSNorm,
 QKV projection with bias, rotary embedding (rotate-half form, theta 1e6), GQA attention
@@ -36,7 +40,10 @@ import torch
 import torch.nn.functional as F
 
 from . import _decode, _lib
+from .batch_tables import batch_tables_buffers, build_batch_tables
 from .int8_cache_write import int8_kv_cache_write
+from .lora import lora_add, lora_plan
+from .sampling import sample_tokens
 
 
 @dataclass(frozen=True)
@@ -350,6 +357,51 @@ def random_weights(shape: QwenShape, device, seed: int = 0, std: float = 0.02,
     return w
 
 
+PROJECTIONS = ("qkv", "o", "gate_up", "down")
+
+
+@dataclass
+class Adapters:
+    """Low-rank adapters of a batch: for each layer the adapted projections' weights, and the
+    adapter of every sequence (a device tensor the captured step reads; -1: none)."""
+
+    ids: torch.Tensor  # [batch] int32 or int64
+    count: int
+    layers: list  # per layer {projection: (lora_a [count, rank, k], lora_b [count, n, rank])}
+    scales: torch.Tensor | None = None  # [count] float32
+
+
+def random_adapters(shape: QwenShape, ids: torch.Tensor, count: int, rank: int,
+                    projections=PROJECTIONS, seed: int = 0, std: float = 0.02) -> Adapters:
+    """Seeded adapters of N(0, std) weights on ``ids``' device."""
+    dev = ids.device
+    g = torch.Generator(device=dev).manual_seed(seed)
+    sizes = {"qkv": (shape.hidden, shape.qkv_width), "o": (shape.q_heads * shape.head_dim, shape.hidden),
+             "gate_up": (shape.hidden, 2 * shape.ffn), "down": (shape.ffn, shape.hidden)}
+
+    def normal(*size):
+        return torch.empty(*size, dtype=torch.bfloat16, device=dev).normal_(0.0, std, generator=g)
+
+    layers = [{name: (normal(count, rank, sizes[name][0]), normal(count, sizes[name][1], rank))
+               for name in projections} for _ in range(shape.layers)]
+    return Adapters(ids, count, layers, torch.rand(count, generator=g, device=dev) * 2)
+
+
+@dataclass
+class Sampling:
+    """Per-sequence settings of ``sample_tokens`` and the random numbers of every generated token."""
+
+    uniforms: torch.Tensor  # [new_tokens, batch] float32
+    temperature: torch.Tensor | None = None  # [batch]; None: 1
+    top_k: torch.Tensor | None = None
+    top_p: torch.Tensor | None = None
+    min_p: torch.Tensor | None = None
+
+    def draw(self, logits: torch.Tensor, uniforms: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
+        return sample_tokens(logits, uniforms, temperature=self.temperature, top_k=self.top_k,
+                             top_p=self.top_p, min_p=self.min_p, out=out)
+
+
 def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
     """Causal GQA attention over [c, H, S, D] bf16 with torch SDPA (flash / memory-efficient).
 
@@ -470,7 +522,8 @@ class DecodeLoop:
     """Prefill + graph-captured greedy decode for one cache mode over a fixed batch."""
 
     def __init__(self, weights: ModelWeights, batch: int, prompt_len: int, new_tokens: int, mode: str,
-                 scales=None, seed: int = 2, device=None):
+                 scales=None, seed: int = 2, device=None, sampling: Sampling | None = None,
+                 adapters: Adapters | None = None, on_demand: bool = False):
         shape = weights.shape
         dev = weights.embed.device if device is None else torch.device(device)
         assert batch >= 1 and prompt_len >= 1 and new_tokens >= 1
@@ -483,6 +536,23 @@ class DecodeLoop:
         g = torch.Generator().manual_seed(seed)
         pool = torch.randperm(self.num_blocks, generator=g).to(torch.int32)
         self.block_tables = pool.view(batch, width).to(dev)
+        # On demand: the pool is a free list, and a step takes a block from it where a sequence's
+        # next token opens one.
+        self.on_demand = on_demand
+        if on_demand:
+            self.free_blocks = pool.to(dev)
+            self.free_head = torch.zeros(1, dtype=torch.int64, device=dev)
+            self.block_tables.fill_(-1)
+            self.one = torch.ones(batch, dtype=torch.int64, device=dev)
+            self.tables = batch_tables_buffers(batch, batch, dev)._replace(free_end=self.free_head)
+        self.sampling, self.adapters = sampling, adapters
+        if sampling is not None:
+            assert sampling.uniforms.shape == (new_tokens, batch), "uniforms: [new_tokens, batch]"
+            self.uniforms = torch.empty(1, batch, dtype=torch.float32, device=dev)
+        if adapters is not None:
+            assert adapters.ids.shape == (batch,) and len(adapters.layers) == shape.layers
+            assert all(name in PROJECTIONS for layer in adapters.layers for name in layer)
+            self.plan = lora_plan(adapters.ids, adapters.count)
         ks, vs = scales if scales is not None else (None, None)
         self.cache = PagedKVCache(shape, self.num_blocks, mode, dev, ks, vs)
         self.cos, self.sin = rope_tables(shape, self.max_len, dev)
@@ -519,40 +589,67 @@ class DecodeLoop:
         bt = self.block_tables[seqs].to(torch.int64)
         return (bt[:, t // BLOCK_SIZE] * BLOCK_SIZE + t % BLOCK_SIZE).reshape(-1)
 
+    def _take_prompt_blocks(self, seqs: slice) -> torch.Tensor:
+        """On demand: gives the sequences the blocks of their prompts; returns the prompts' slots."""
+        rows = self.block_tables[seqs]
+        n, S = rows.shape[0], self.prompt_len
+        lens = torch.zeros(n, dtype=torch.int64, device=self.dev)
+        out = batch_tables_buffers(n, n * S, self.dev)._replace(free_end=self.free_head)
+        return build_batch_tables(lens, lens + S, rows, self.free_blocks, n * S, block_size=BLOCK_SIZE,
+                                  free_start=self.free_head, out=out).slot_mapping
+
+    def _adapt(self, name: str, layer: int, x: torch.Tensor, out: torch.Tensor, plan) -> torch.Tensor:
+        """Adds the layer's adapters of one projection of x to its output, in place."""
+        if plan is not None and name in self.adapters.layers[layer]:
+            a, b = self.adapters.layers[layer][name]
+            lora_add(out, x, a, b, plan, scales=self.adapters.scales, out=out)
+        return out
+
     def prefill(self, prompt_ids: torch.Tensor, chunk_tokens: int = 32768) -> torch.Tensor:
         """Runs the prompt [B, S] through the model, fills the caches, returns the first tokens."""
         shape, B, S = self.shape, self.batch, self.prompt_len
         Hq, Hkv, D, L = shape.q_heads, shape.kv_heads, shape.head_dim, shape.layers
         assert prompt_ids.shape == (B, S)
         ids = prompt_ids.to(self.dev)
+        if self.on_demand:
+            self.block_tables.fill_(-1)
+            self.free_head.zero_()
         c = max(1, min(B, chunk_tokens // S))
         last = torch.empty(B, shape.hidden, dtype=torch.bfloat16, device=self.dev)
         with torch.inference_mode():
             for b0 in range(0, B, c):
                 sl = slice(b0, min(B, b0 + c))
                 n = sl.stop - sl.start
-                slots = self.prefill_slots(sl)
+                slots = self._take_prompt_blocks(sl) if self.on_demand else self.prefill_slots(sl)
                 pos = torch.arange(S, device=self.dev).repeat(n)
+                plan = None
+                if self.adapters is not None:
+                    plan = lora_plan(self.adapters.ids[sl].repeat_interleave(S), self.adapters.count)
                 x = F.embedding(ids[sl].reshape(-1), self.w.embed)
                 h = torch.empty_like(x)
                 hip_add_rms_norm(x, None, self.w.layers[0].ln1, h, shape.rms_eps)
                 for l, lw in enumerate(self.w.layers):
-                    qkv = F.linear(h, lw.wqkv, lw.bqkv)
+                    qkv = self._adapt("qkv", l, h, F.linear(h, lw.wqkv, lw.bqkv), plan)
                     hip_rotary_(qkv, Hq + Hkv, D, pos, self.cos, self.sin)
                     q, k, v = _split_qkv(qkv, shape)
                     self.cache.write(l, k, v, slots)
                     attn = prefill_attention(*(t.view(n, S, -1, D).transpose(1, 2).contiguous()
                                                for t in (q, k, v)))
                     attn = attn.transpose(1, 2).reshape(n * S, Hq * D)
-                    hip_add_rms_norm(x, F.linear(attn, lw.wo), lw.ln2, h, shape.rms_eps)
-                    gu = F.linear(h, lw.w_gate_up)
+                    hip_add_rms_norm(x, self._adapt("o", l, attn, F.linear(attn, lw.wo), plan), lw.ln2,
+                                     h, shape.rms_eps)
+                    gu = self._adapt("gate_up", l, h, F.linear(h, lw.w_gate_up), plan)
                     act = hip_silu_mul(gu, torch.empty(n * S, shape.ffn, dtype=x.dtype, device=self.dev))
                     del gu
                     nxt = self.w.layers[l + 1].ln1 if l + 1 < L else self.w.ln_f
-                    hip_add_rms_norm(x, F.linear(act, lw.w_down), nxt, h, shape.rms_eps)
+                    hip_add_rms_norm(x, self._adapt("down", l, act, F.linear(act, lw.w_down), plan), nxt,
+                                     h, shape.rms_eps)
                 last[sl] = h.view(n, S, shape.hidden)[:, -1]
             logits = F.linear(last, self.w.lm_head)
-            first = logits.argmax(-1)
+            if self.sampling is None:
+                first = logits.argmax(-1)
+            else:
+                first = self.sampling.draw(logits, self.sampling.uniforms[0], torch.empty_like(self.tokens))
         self.prefill_logits = logits
         self.tokens.copy_(first)
         self.generated[:, 0].copy_(first)
@@ -571,6 +668,12 @@ class DecodeLoop:
         shape, B = self.shape, self.batch
         Hq, D, L = shape.q_heads, shape.head_dim, shape.layers
         pos = self.positions
+        if self.on_demand:
+            build_batch_tables(pos, self.one, self.block_tables, self.free_blocks, B,
+                               block_size=BLOCK_SIZE, free_start=self.free_head, out=self.tables)
+        plan = None
+        if self.adapters is not None:
+            plan = lora_plan(self.adapters.ids, self.adapters.count, plan=self.plan)
         if not FUSED_STEP:
             slots = self.block_tables.gather(1, (pos // BLOCK_SIZE).view(B, 1)).view(B).to(torch.int64)
             slots = slots * BLOCK_SIZE + pos % BLOCK_SIZE
@@ -579,10 +682,22 @@ class DecodeLoop:
         hip_add_rms_norm(x, None, self.w.layers[0].ln1, h, shape.rms_eps)
         for l, lw in enumerate(self.w.layers):
             skinny = self._skinny(lw.wqkv, lw.wo, lw.w_gate_up, lw.w_down)
+            adapted = {} if plan is None else self.adapters.layers[l]
+
+            def project(name, x_in, w, bias=None):
+                """A projection with its adapters, where no fused form of it applies."""
+                if skinny:
+                    out = torch.empty(B, w.shape[0], dtype=x_in.dtype, device=self.dev)
+                    hip_linear(x_in, w, bias, out, self.partials)
+                else:
+                    out = F.linear(x_in, w, bias)
+                return self._adapt(name, l, x_in, out, plan)
+
             if skinny:
                 qkv = hip_linear(h, lw.wqkv, lw.bqkv, self.qkv, self.partials)
             else:
                 qkv = F.linear(h, lw.wqkv, lw.bqkv)
+            self._adapt("qkv", l, h, qkv, plan)
             if FUSED_STEP:
                 self.cache.rotary_write(l, qkv, pos, self.cos, self.sin, self.block_tables)
                 q, _, _ = _split_qkv(qkv, shape)
@@ -593,19 +708,27 @@ class DecodeLoop:
             self.cache.attend(l, q, self.block_tables, self.seq_lens, self.attn_out, self.workspace)
             attn = self.attn_out.view(B, Hq * D)
             nxt = self.w.layers[l + 1].ln1 if l + 1 < L else self.w.ln_f
-            if skinny:
+            if skinny and "o" not in adapted:
                 hip_linear_add_rms_norm(attn, lw.wo, x, lw.ln2, h, shape.rms_eps, self.partials)
+            else:
+                hip_add_rms_norm(x, project("o", attn, lw.wo), lw.ln2, h, shape.rms_eps)
+            if skinny and "gate_up" not in adapted:
                 hip_linear_silu_mul(h, lw.w_gate_up, self.act)
+            else:
+                hip_silu_mul(project("gate_up", h, lw.w_gate_up), self.act)
+            if skinny and "down" not in adapted:
                 hip_linear_add_rms_norm(self.act, lw.w_down, x, nxt, h, shape.rms_eps, self.partials)
             else:
-                hip_add_rms_norm(x, F.linear(attn, lw.wo), lw.ln2, h, shape.rms_eps)
-                hip_silu_mul(F.linear(h, lw.w_gate_up), self.act)
-                hip_add_rms_norm(x, F.linear(self.act, lw.w_down), nxt, h, shape.rms_eps)
+                hip_add_rms_norm(x, project("down", self.act, lw.w_down), nxt, h, shape.rms_eps)
         if self._skinny(self.w.lm_head):
             hip_linear(h, self.w.lm_head, None, self.logits, self.partials)
         else:
             torch.mm(h, self.w.lm_head.t(), out=self.logits)
-        if FUSED_STEP:
+        if self.sampling is not None:
+            torch.index_select(self.sampling.uniforms, 0, self.step_idx.clamp(max=self.new_tokens - 1),
+                               out=self.uniforms)
+            self.sampling.draw(self.logits, self.uniforms[0], self.tokens)
+        elif FUSED_STEP:
             hip_argmax_rows(self.logits, self.tokens)
         else:
             self.tokens.copy_(self.logits.argmax(-1))
@@ -615,11 +738,15 @@ class DecodeLoop:
         self.seq_lens.add_(1)
         self.step_idx.add_(1)
 
+    def _state(self):
+        state = [self.tokens, self.positions, self.seq_lens, self.step_idx, self.generated]
+        return state + [self.block_tables, self.free_head] if self.on_demand else state
+
     def state(self):
-        return [t.clone() for t in (self.tokens, self.positions, self.seq_lens, self.step_idx, self.generated)]
+        return [t.clone() for t in self._state()]
 
     def restore(self, saved) -> None:
-        for dst, src in zip((self.tokens, self.positions, self.seq_lens, self.step_idx, self.generated), saved):
+        for dst, src in zip(self._state(), saved):
             dst.copy_(src)
 
     def step_eager(self) -> None:
