@@ -37,6 +37,7 @@ constexpr int kMaxTiles = kThreads;    // one per thread in the tile scan
 constexpr int kList = 4096;            // tokens a row's exact order is made of
 constexpr int64_t kMaxVocab = 1 << 21;  // 513 chunks at most
 constexpr int64_t kMaxRows = 1 << 16;
+constexpr int64_t kGroupRows = 1024;  // rows that share a workspace (60 KB each) and its launches
 
 struct SampleArgs {
   const void* logits;
@@ -621,7 +622,7 @@ __device__ __forceinline__ float nucleus_from(const SampleArgs& a, const Params&
   if (top == INFINITY) return top;
   const double z = (double)total * __longlong_as_double((int64_t)(1023 - a.frac) << 52);
   const double d = -log((1.0 - q.p) * z / (double)a.vocab) * (double)q.t * (1.0 + 0x1p-20);
-  return d > 0.0 ? (float)((double)top - d) - fabsf(top) * 0x1p-20f : top;
+  return d > 0.0 ? (float)((double)top - d) - (fabsf(top) + (float)d) * 0x1p-20f : top;
 }
 
 template <int DT>
@@ -1368,12 +1369,13 @@ __device__ __forceinline__ int32_t nucleus_bin(const Params& q, uint64_t total,
   return bin;
 }
 
-// The smallest value of a bin, or a little less.
+// The smallest value of a bin, or a little less (d is rounded, and so is the value from it: both
+// errors are relative to d or to top, whichever is larger).
 __device__ __forceinline__ float bin_from(int32_t bin, float top) {
   if (bin >= kBins - 1) return -INFINITY;
   if (top == INFINITY) return top;
   const float d = __uint_as_float((uint32_t)(bin + kBinBase) << kBinShift);  // the next bin's least d
-  return (float)((double)top - (double)d) - fabsf(top) * 0x1p-20f;
+  return (float)((double)top - (double)d) - (fabsf(top) + d) * 0x1p-20f;
 }
 
 struct GatherShared {
@@ -1533,7 +1535,7 @@ __global__ __launch_bounds__(kThreads) void row_kernel(SampleArgs a) {
     } else {
       // min-p alone: w >= m is M - v <= -T ln m (and a little more, for the roundings).
       const double d = -log(q.m) * (double)q.t * (1.0 + 0x1p-20) + 0x1p-100;
-      last = bin_of((float)((double)top - d) - fabsf(top) * 0x1p-20f, top);
+      last = bin_of((float)((double)top - d) - (fabsf(top) + (float)d) * 0x1p-20f, top);
     }
     if (confirmed && tile_max >= bin_from(last, top) && tile_max > -INFINITY)
       s.visit[atomicAdd(&s.visits, 1)] = t;
@@ -1645,12 +1647,33 @@ void launch_sample(const SampleArgs& a, hipStream_t s) {
   hipLaunchKernelGGL(row_kernel<DT>, dim3((unsigned)a.rows), dim3(kThreads), 0, s, a);
 }
 
+// How the passes of a.rows rows are cut.
+void plan_launches(SampleArgs& a) {
+  // Runs of chunks long enough for the loads of one to hide behind the weights of another, while
+  // there are enough of them to fill the compute units.
+  const int64_t per_unit = a.rows * a.chunks / 2048;
+  a.run_chunks = (int32_t)(per_unit < 1 ? 1 : (per_unit < 8 ? per_unit : 8));
+  a.runs = (a.chunks + a.run_chunks - 1) / a.run_chunks;
+  // The histogram pass and the gathering behind it run where some row may have a nucleus cut alone
+  // and more tokens than its list holds.  A compute unit takes one of their workgroups; parts for
+  // twice the units, since rows with other settings leave at once (61 rows of mixed settings: 13 us
+  // each with 8 parts, 18 with 4), unless two rows out of three would wait for a second turn (200
+  // rows, all with a nucleus cut: 23 and 19 us with 1 part, 25 and 23 with 2).
+  a.parts = 0;
+  if (a.top_p && a.pieces > kList / kPieceElements) {
+    const int64_t most = (a.vocab + 4 * kThreads - 1) / (4 * kThreads);
+    const int64_t want = a.rows <= 128 ? 512 / a.rows : (256 / a.rows < 1 ? 1 : 256 / a.rows);
+    a.parts = (int32_t)(want < most ? want : most);
+  }
+}
+
 }  // namespace
 
 extern "C" size_t int8kv_sample_workspace_bytes(int64_t rows, int64_t vocab) {
   if (rows < 0 || rows > kMaxRows || vocab < 1 || vocab > kMaxVocab) return 0;
   const int64_t chunks = chunks_of(vocab, true);  // at least those of the 16-bit types
-  return (size_t)workspace_of(rows > 0 ? rows : 1, chunks, nullptr, nullptr);
+  const int64_t group = rows < kGroupRows ? rows : kGroupRows;
+  return (size_t)workspace_of(group > 0 ? group : 1, chunks, nullptr, nullptr);
 }
 
 extern "C" int int8kv_sample_rows(const void* logits, int logits_dtype, int64_t rows, int64_t vocab,
@@ -1668,41 +1691,31 @@ extern "C" int int8kv_sample_rows(const void* logits, int logits_dtype, int64_t 
   if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 ||
       workspace_bytes < int8kv_sample_workspace_bytes(rows, vocab))
     return INT8KV_E_WORKSPACE;
-  SampleArgs a;
-  a.logits = logits;
-  a.rows = rows;
-  a.row_stride = row_stride;
-  a.vocab = (int32_t)vocab;
-  a.frac = frac_bits(vocab);
-  a.u = uniforms;
-  a.temperature = temperature;
-  a.top_k = top_k;
-  a.top_p = top_p;
-  a.min_p = min_p;
-  a.out = out;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  workspace_of(rows, chunks_of(vocab, logits_dtype == INT8KV_F32), &a, static_cast<char*>(workspace));
-  // Runs of chunks long enough for the loads of one to hide behind the weights of another, while
-  // there are enough of them to fill the compute units.
-  const int64_t per_unit = rows * a.chunks / 2048;
-  a.run_chunks = (int32_t)(per_unit < 1 ? 1 : (per_unit < 8 ? per_unit : 8));
-  a.runs = (a.chunks + a.run_chunks - 1) / a.run_chunks;
-  // The histogram pass and the gathering behind it run where some row may have a nucleus cut alone
-  // and more tokens than its list holds.  A compute unit takes one of their workgroups; parts for
-  // twice the units, since rows with other settings leave at once (61 rows of mixed settings: 13 us
-  // each with 8 parts, 18 with 4), unless two rows out of three would wait for a second turn (200
-  // rows, all with a nucleus cut: 23 and 19 us with 1 part, 25 and 23 with 2).
-  a.parts = 0;
-  if (top_p && a.pieces > kList / kPieceElements) {
-    const int64_t most = (vocab + 4 * kThreads - 1) / (4 * kThreads);
-    const int64_t want = rows <= 128 ? 512 / rows : (256 / rows < 1 ? 1 : 256 / rows);
-    a.parts = (int32_t)(want < most ? want : most);
+  for (int64_t r0 = 0; r0 < rows; r0 += kGroupRows) {
+    const int64_t n = rows - r0 < kGroupRows ? rows - r0 : kGroupRows;
+    SampleArgs a;
+    a.logits = static_cast<const char*>(logits) + r0 * row_stride * (int64_t)size;
+    a.rows = n;
+    a.row_stride = row_stride;
+    a.vocab = (int32_t)vocab;
+    a.frac = frac_bits(vocab);
+    a.u = uniforms + r0;
+    a.temperature = temperature ? temperature + r0 : nullptr;
+    a.top_k = top_k ? top_k + r0 : nullptr;
+    a.top_p = top_p ? top_p + r0 : nullptr;
+    a.min_p = min_p ? min_p + r0 : nullptr;
+    a.out = out + r0;
+    workspace_of(n, chunks_of(vocab, logits_dtype == INT8KV_F32), &a, static_cast<char*>(workspace));
+    plan_launches(a);
+    if (logits_dtype == INT8KV_F32)
+      launch_sample<kF32>(a, s);
+    else if (logits_dtype == INT8KV_BF16)
+      launch_sample<kBF16>(a, s);
+    else
+      launch_sample<kF16>(a, s);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return (int)e;
   }
-  if (logits_dtype == INT8KV_F32)
-    launch_sample<kF32>(a, s);
-  else if (logits_dtype == INT8KV_BF16)
-    launch_sample<kBF16>(a, s);
-  else
-    launch_sample<kF16>(a, s);
-  return (int)hipGetLastError();
+  return INT8KV_OK;
 }

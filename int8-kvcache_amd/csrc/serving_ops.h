@@ -49,7 +49,8 @@ extern "C" {
  *
  *   computed_lens, new_lens: [requests] of lens_dtype (I32 or I64), contiguous.  block_tables:
  *   int32 [requests, table_width], unit inner stride.  free_blocks: int32 [num_free].
- *   free_start: one int64 on the device, or NULL for 0; free_end may be the same location.
+ *   free_start: one int64 on the device, or NULL for 0; free_end may be the same location.  No
+ *   other output may overlap an input.
  *   workspace: int8kv_batch_tables_workspace_bytes(requests) bytes, 16-byte aligned, no
  *   initialisation needed; calls that share one must not overlap.  block_size in [1, 65536].
  */

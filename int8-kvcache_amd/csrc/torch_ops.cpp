@@ -322,6 +322,9 @@ void build_batch_tables(at::Tensor computed_lens, at::Tensor new_lens, const at:
   }
   const auto buffer = [&](const at::Tensor& t, at::ScalarType type, int64_t n) {
     require(t.scalar_type() == type && t.is_contiguous() && t.numel() == n);
+    require(requests == 0 || n == 0 || (t.data_ptr() != computed_lens.data_ptr() &&
+                                        t.data_ptr() != new_lens.data_ptr()),
+            "an output shares memory with the lengths");
   };
   buffer(query_starts, at::kInt, requests + 1);
   buffer(seq_lens, at::kInt, requests);

@@ -63,7 +63,8 @@ def build_batch_tables(
     do not fit are dropped as if their request brought fewer.
 
     A token's slot is -1 where its block lies past the table's width or the free list ran out
-    (``free_end`` then exceeds ``free_blocks.numel()``).  ``out.free_end`` may be ``free_start`` itself.
+    (``free_end`` then exceeds ``free_blocks.numel()``).  ``out.free_end`` may be ``free_start`` itself;
+    no other output may share memory with an input.
     """
     ext = None if _decode.DEBUG_CHECKS else _ext.module()
     if ext is not None:
@@ -95,6 +96,9 @@ def build_batch_tables(
     for t, dtype, size in zip(out, _OUT_DTYPES, sizes):
         assert t.dtype == dtype and t.is_contiguous() and t.numel() == size
     assert all(t.device == dev for t in [*given, *out]), "all tensors must be on one device (the GPU)"
+    lens = {computed_lens.data_ptr(), new_lens.data_ptr()}
+    assert not requests or not any(t.numel() and t.data_ptr() in lens for t in out), \
+        "an output shares memory with the lengths"
     if _decode.DEBUG_CHECKS:
         _debug_check(computed_lens, new_lens, block_tables, free_blocks, num_tokens, block_size,
                      free_start)

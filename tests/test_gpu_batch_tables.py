@@ -114,6 +114,18 @@ def test_odd_lengths(cuda):
     check(*run(case, cuda, 20, start=0))
 
 
+def test_outputs_over_the_lengths_are_refused(cuda):
+    lens = torch.ones(4, dtype=torch.int32, device=cuda)
+    tables = torch.zeros(4, 3, dtype=torch.int32, device=cuda)
+    free = torch.arange(9, dtype=torch.int32, device=cuda)
+    out = int8kv.batch_tables_buffers(4, 4, cuda)
+    for bad in (out._replace(seq_lens=lens), out._replace(token_requests=lens)):
+        with pytest.raises(AssertionError, match="shares memory"):
+            int8kv.build_batch_tables(lens, lens.clone(), tables, free, 4, out=bad)
+        with _ext.use_ctypes(), pytest.raises(AssertionError, match="shares memory"):
+            int8kv.build_batch_tables(lens, lens.clone(), tables, free, 4, out=bad)
+
+
 def test_no_requests(cuda):
     case = dict(c=np.zeros(0, np.int64), n=np.zeros(0, np.int64), tables=np.zeros((0, 4), np.int64),
                 free=np.arange(3), dtype=torch.int32, bs=16)

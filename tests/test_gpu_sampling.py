@@ -158,6 +158,28 @@ def test_live_tokens_in_few_places(cuda):
             both(cuda, logits, u, **kw)
 
 
+def test_log_probabilities(cuda):
+    """Rows whose maximum is close to zero while the cut lies far below it, at every distance."""
+    g = torch.Generator().manual_seed(17)
+    for dtype in DTYPES:
+        for spread, shift in ((3.0, 0.0), (40.0, 1e-3), (0.5, -1e-4)):
+            logits = torch.log_softmax(torch.randn(24, 30011, generator=g) * spread, -1)
+            logits = (logits - logits.amax(-1, keepdim=True) + shift).to(dtype)
+            u = torch.rand(24, generator=g)
+            t = spread / 3 if spread > 1 else 1.0
+            for kw in ({"top_k": 100}, {"top_k": 1000}, {"top_p": 0.95}, {"top_p": 0.6, "min_p": 0.01},
+                       {"min_p": 1e-3}, {}):
+                both(cuda, logits, u, temperature=t, **kw)
+
+
+def test_more_rows_than_share_a_workspace(cuda):
+    logits, u = random_logits(2500, 5003, torch.bfloat16, seed=18)
+    for kw in ({}, {"top_p": 0.9}, {"top_k": 30, "top_p": 0.9}):
+        both(cuda, logits, u, **kw)
+    ks = [0, 1, 50] * 833 + [7]
+    both(cuda, logits, u, top_k=ks, top_p=0.8, temperature=0.7)
+
+
 def test_vocabularies_of_more_pieces_than_tiles(cuda):
     for vocab in (262145, 400003, 2**21):
         logits, u = random_logits(2, vocab, torch.bfloat16, seed=vocab)
