@@ -404,10 +404,21 @@ __global__ __launch_bounds__(kChunkThreads) void chunk_kernel(SampleArgs a) {
   }
 }
 
-// The row's maximum from its chunks' (one value per thread; s_max: kWaves).
-__device__ __forceinline__ float row_max(const SampleArgs& a, int64_t r, float* s_max) {
-  float m = (int32_t)threadIdx.x < a.chunks ? a.chunk_max[r * a.chunks + threadIdx.x] : -INFINITY;
-  m = wave_max(m);
+// One chunk per thread: its maximum, and its mass in units of that (where it was summed).
+struct Chunk {
+  float top;
+  uint64_t mass;
+};
+__device__ __forceinline__ Chunk own_chunk(const SampleArgs& a, int64_t r) {
+  const int64_t i = r * a.chunks + ((int32_t)threadIdx.x < a.chunks ? (int32_t)threadIdx.x : 0);
+  Chunk c{a.chunk_max[i], a.chunk_mass[i]};
+  if ((int32_t)threadIdx.x >= a.chunks) c = Chunk{-INFINITY, 0};
+  return c;
+}
+
+// The row's maximum from its chunks' (s_max: kWaves).
+__device__ __forceinline__ float row_max(const Chunk& chunk, float* s_max) {
+  float m = wave_max(chunk.top);
   if ((threadIdx.x & 63) == 0) s_max[threadIdx.x >> 6] = m;
   __syncthreads();
 #pragma unroll
@@ -415,23 +426,16 @@ __device__ __forceinline__ float row_max(const SampleArgs& a, int64_t r, float* 
   return m;
 }
 
-// The row's mass from its chunks', each scaled from its own maximum to the row's (one chunk per
-// thread): returns the mass before this thread's chunk; `factor` is its scale.
-__device__ __forceinline__ uint64_t scan_chunks(const SampleArgs& a, int64_t r, const Params& q,
-                                                float top, uint64_t* s_wave, float& chunk_top,
-                                                uint64_t& own, uint64_t& mass, double& factor,
+// The row's mass from its chunks', each scaled from its own maximum to the row's: returns the mass
+// before this thread's chunk, `mass` its own and `factor` its scale.
+__device__ __forceinline__ uint64_t scan_chunks(const Chunk& chunk, const Params& q, float top,
+                                                uint64_t* s_wave, uint64_t& mass, double& factor,
                                                 uint64_t& total) {
-  const int32_t t = threadIdx.x;
-  own = mass = 0;
+  mass = chunk.mass;
   factor = 1.0;
-  chunk_top = -INFINITY;
-  if (t < a.chunks) {
-    chunk_top = a.chunk_max[r * a.chunks + t];
-    mass = own = a.chunk_mass[r * a.chunks + t];
-    if (chunk_top < top) {
-      factor = exp2(fmax(((double)chunk_top - (double)top) * (0x1.71547652b82fep+0 / (double)q.t), -200.0));
-      mass = (uint64_t)rint((double)own * factor);
-    }
+  if (mass > 0 && chunk.top < top) {
+    factor = exp2(fmax(((double)chunk.top - (double)top) * (0x1.71547652b82fep+0 / (double)q.t), -200.0));
+    mass = (uint64_t)rint((double)mass * factor);
   }
   return workgroup_scan<kWaves, uint64_t>(mass, s_wave, total);
 }
@@ -637,14 +641,14 @@ __global__ __launch_bounds__(kThreads) void bins_kernel(SampleArgs a) {
   const int32_t per = (tiles.count + a.parts - 1) / a.parts;
   const int32_t tile = part * per + t;
   const float tile_max = t < per && tile < tiles.count ? tiles.max_of(a, r, tile) : -INFINITY;
+  const Chunk chunk = own_chunk(a, r);
   for (int32_t b = t; b < 2 * kBins; b += kThreads) s.mass[b] = 0;
   if (t == 0) s.visits = s.queue.length = 0;
-  const float top = row_max(a, r, s.wave_max);
+  const float top = row_max(chunk, s.wave_max);
   if (top == -INFINITY) return;
-  float chunk_top;
-  uint64_t own, mass, total;
+  uint64_t mass, total;
   double factor;
-  scan_chunks(a, r, q, top, s.wave64, chunk_top, own, mass, factor, total);
+  scan_chunks(chunk, q, top, s.wave64, mass, factor, total);
   const float from = nucleus_from(a, q, top, total);
   if (tile_max >= from && tile_max > -INFINITY) s.visit[atomicAdd(&s.visits, 1)] = tile;
   __syncthreads();
@@ -1033,7 +1037,7 @@ __device__ __forceinline__ bool cut_by_bins(const Weights& w, const Params& q, c
   uint64_t mass_all = 0, mb = 0;
   const uint32_t cb = workgroup_scan<kWaves, uint32_t>(c0 + c1, s.wave32, count_all);
   if (q.p < 1.0) mb = workgroup_scan<kWaves, uint64_t>(m0 + m1, s.wave64, mass_all);
-  const bool top_k = q.k > 0 && q.k < n;
+  const bool top_k = q.k > 0 && q.k <= n;  // (n: the row may have more tokens than its list)
   uint64_t kept = mass_all;
   last = 0;  // (everything)
   int32_t count;
@@ -1138,8 +1142,9 @@ __device__ __forceinline__ int32_t pick_in_slots(const Row<DT>& row, int32_t s0,
 
 // Rows without a filter: the chunk that holds the target from the chunks' masses, then the token.
 template <int DT>
-__device__ __forceinline__ void finish_plain(const SampleArgs& a, const Row<DT>& row, int64_t r, const Params& q,
-                             float top, RowShared& s) {
+__device__ __forceinline__ void finish_plain(const SampleArgs& a, const Row<DT>& row, int64_t r,
+                                             const Params& q, const Chunk& chunk, float top,
+                                             RowShared& s) {
   constexpr int kE = Row<DT>::kE;
   constexpr int kChunkSlots = kChunkElements / kE;  // at most kThreads
   const int t = threadIdx.x;
@@ -1148,17 +1153,16 @@ __device__ __forceinline__ void finish_plain(const SampleArgs& a, const Row<DT>&
     s.value64[0] = 0;
     s.value32[0] = 0;
   }
-  float m;
-  uint64_t own, mass, total;
+  uint64_t mass, total;
   double factor;
-  const uint64_t before = scan_chunks(a, r, q, top, s.wave64, m, own, mass, factor, total);
+  const uint64_t before = scan_chunks(chunk, q, top, s.wave64, mass, factor, total);
   const uint64_t target = scaled(q.u, total);
   if (before <= target && target < before + mass) {  // one thread
     uint64_t left = target - before;
-    if (m < top) left = (uint64_t)((double)left / factor);
-    s.value64[0] = left < own ? left : own - 1;
+    if (chunk.top < top) left = (uint64_t)((double)left / factor);
+    s.value64[0] = left < chunk.mass ? left : chunk.mass - 1;
     s.value32[0] = t;
-    s.wave_max[0] = m;
+    s.wave_max[0] = chunk.top;
   }
   __syncthreads();
   // The chunk's slots, one per thread.
@@ -1410,17 +1414,17 @@ __global__ __launch_bounds__(kThreads) void gather_kernel(SampleArgs a) {
   if (tile0 >= tile1) return;
   for (int32_t b = t; b < kBins; b += kThreads) s.bin_mass[b] = a.bin_mass[r * kBins + b];
   const float tile_max = t < tile1 - tile0 ? tiles.max_of(a, r, tile0 + t) : -INFINITY;
+  const Chunk chunk = own_chunk(a, r);
   if (t == 0) s.visits = s.length = 0;
   s.tile_mass[t] = 0;
-  const float top = row_max(a, r, s.wave_max);  // (with a barrier)
+  const float top = row_max(chunk, s.wave_max);  // (with a barrier)
   if (top == -INFINITY) return;
   const Row<DT> row(a, r);
   const Weights w{0x1.71547652b82fep+0 / (double)q.t, (double)top, top, a.frac};
   const uint64_t least = least_weight(q.m, a.frac);
-  float chunk_top;
-  uint64_t own, mass, total, before, binned;
+  uint64_t mass, total, before, binned;
   double factor;
-  scan_chunks(a, r, q, top, s.wave64, chunk_top, own, mass, factor, total);
+  scan_chunks(chunk, q, top, s.wave64, mass, factor, total);
   const int32_t bin = nucleus_bin(q, total, s.bin_mass, s, before, binned);
   const float from = bin_from(bin, top);
   if (t == 0) s.queue.length = 0;
@@ -1466,6 +1470,7 @@ __global__ __launch_bounds__(kThreads) void row_kernel(SampleArgs a) {
   const bool filter = q.k > 0 || q.p < 1.0;
   const bool counted = needs_bins(a, q);  // histogram and list are there
   const float tile_max = t < tiles.count ? tiles.max_of(a, r, t) : -INFINITY;
+  const Chunk chunk = own_chunk(a, r);
   s.tile_mass[t] = counted && t < tiles.count ? a.tile_mass[r * kMaxTiles + t] : 0;
   if (filter)
     for (int32_t b = t; b < kBins; b += kThreads) {
@@ -1479,7 +1484,7 @@ __global__ __launch_bounds__(kThreads) void row_kernel(SampleArgs a) {
     s.visits = s.queue.length = 0;
     s.value32[4] = kMaxTiles;  // first tile with the maximum
   }
-  const float top = row_max(a, r, s.wave_max);
+  const float top = row_max(chunk, s.wave_max);
   __syncthreads();
   if (top == -INFINITY) {
     if (t == 0) a.out[r] = 0;
@@ -1499,7 +1504,7 @@ __global__ __launch_bounds__(kThreads) void row_kernel(SampleArgs a) {
     return;
   }
   if (!filter && !(q.m > 0.0)) {
-    finish_plain(a, row, r, q, top, s);
+    finish_plain(a, row, r, q, chunk, top, s);
     return;
   }
   const Weights w{0x1.71547652b82fep+0 / (double)q.t, (double)top, top, a.frac};
@@ -1507,16 +1512,16 @@ __global__ __launch_bounds__(kThreads) void row_kernel(SampleArgs a) {
   ListCut cut{0, 0};
   bool confirmed = true;
   if (counted) {
-    float chunk_top;
-    uint64_t own, mass, total, binned;
+    uint64_t mass, total, binned;
     double factor;
-    scan_chunks(a, r, q, top, s.wave64, chunk_top, own, mass, factor, total);
+    scan_chunks(chunk, q, top, s.wave64, mass, factor, total);
     nucleus_bin(q, total, s.list.bin_mass, s, cut.before, binned);
     cut.all_mass = total < binned ? binned : total;
     const int32_t n = s.length < kList ? s.length : kList;
     for (int32_t i = t; i < n; i += kThreads) s.list.place[i] = a.list[r * kList + i];
   } else {
     int32_t last = kBins - 1;
+    bool counting = false;
     if (filter) {
       if (tile_max > -INFINITY) atomicAdd(&s.list.bin_count[bin_of(tile_max, top)], 1u);
       const uint32_t live = (uint32_t)__syncthreads_count(tile_max > -INFINITY);
@@ -1529,33 +1534,62 @@ __global__ __launch_bounds__(kThreads) void row_kernel(SampleArgs a) {
           rank = (uint32_t)ceilf((float)live * share);
           rank = rank < live ? rank : live;
         }
-        last = find_bin<uint32_t>(s.list.bin_count, rank, s.wave32, s, before, all);
         confirmed = k <= kList;  // (no list could hold it)
+        counting = k > 3 * live;
+        if (!counting) last = find_bin<uint32_t>(s.list.bin_count, rank, s.wave32, s, before, all);
       }
     } else {
       // min-p alone: w >= m is M - v <= -T ln m (and a little more, for the roundings).
       const double d = -log(q.m) * (double)q.t * (1.0 + 0x1p-20) + 0x1p-100;
       last = bin_of((float)((double)top - d) - (fabsf(top) + (float)d) * 0x1p-20f, top);
     }
-    if (confirmed && tile_max >= bin_from(last, top) && tile_max > -INFINITY)
-      s.visit[atomicAdd(&s.visits, 1)] = t;
-    __syncthreads();
-    // (min-p alone lists nothing: its tokens' weights go to their tiles.)
-    read_tiles_sparse(row, tiles, s.visit, s.visits, bin_from(last, top), s.queue,
-                      [&](float v, int32_t index) {
-      if (filter) {
-        if (bin_of(v, top) > last) return;
-        const int32_t at = atomicAdd(&s.length, 1);
-        if (at < kList) s.list.place[at] = place_of(key_of(v), index);
-      } else {
-        const uint64_t x = w(v);
-        if (x >= least && x > 0)
-          atomicAdd(reinterpret_cast<unsigned long long*>(&s.tile_mass[tiles.of(row, index)]),
-                    (unsigned long long)x);
+    // A guess that was too high or too low is followed by a count of the row's tokens per bin, and
+    // that by the list down to the bin of the k-th.
+    for (int turn = counting ? 1 : 0; confirmed; ++turn) {
+      if (counting) {
+        __syncthreads();
+        for (int32_t b = t; b < kBins; b += kThreads) s.list.bin_count[b] = 0;
       }
-    });
-    // The list holds the first k tokens, or every live one.
-    confirmed = confirmed && (last == kBins - 1 || !filter || s.length >= q.k);
+      const float from = bin_from(last, top);
+      if (tile_max >= from && tile_max > -INFINITY) s.visit[atomicAdd(&s.visits, 1)] = t;
+      __syncthreads();
+      // (min-p alone lists nothing: its tokens' weights go to their tiles.)
+      read_tiles_sparse(row, tiles, s.visit, s.visits, from, s.queue, [&](float v, int32_t index) {
+        if (filter) {
+          const int32_t b = bin_of(v, top);
+          if (b > last) return;
+          if (counting) {
+            atomicAdd(&s.list.bin_count[b], 1u);
+            return;
+          }
+          const int32_t at = atomicAdd(&s.length, 1);
+          if (at < kList) s.list.place[at] = place_of(key_of(v), index);
+        } else {
+          const uint64_t x = w(v);
+          if (x >= least && x > 0)
+            atomicAdd(reinterpret_cast<unsigned long long*>(&s.tile_mass[tiles.of(row, index)]),
+                      (unsigned long long)x);
+        }
+      });
+      if (!filter) break;
+      if (counting) {
+        uint32_t before, all;
+        const int32_t bin = find_bin<uint32_t>(s.list.bin_count, (uint32_t)q.k, s.wave32, s, before, all);
+        last = bin < last ? bin : last;  // (kBins: fewer than k tokens in all)
+        counting = false;
+      } else {
+        // The list holds the first k tokens, or every live one.
+        const int32_t n = s.length;
+        const bool enough = last == kBins - 1 || n >= q.k;
+        if (n <= kList && enough) break;
+        confirmed = turn == 0 && q.k > 0;
+        counting = true;
+        if (!enough) last = kBins - 1;
+      }
+      __syncthreads();
+      if (t == 0) s.length = s.visits = s.queue.length = 0;
+      __syncthreads();
+    }
   }
   __syncthreads();
   uint64_t last_place = 0;

@@ -128,6 +128,22 @@ def test_dense_values_at_the_cut(cuda):
             both(cuda, logits, u, **kw)
 
 
+def test_as_many_as_top_k_stand_apart(cuda):
+    """k tokens far above the others, k from a short order to a long one: the cut ends with them."""
+    g = torch.Generator().manual_seed(15)
+    for dtype in DTYPES:
+        for vocab in (5003, 32000):
+            for k in (200, 257, 700, 3001, 4096):
+                logits = torch.randn(24, vocab, generator=g)
+                for r in range(24):
+                    at = torch.randperm(vocab, generator=g)[:k]
+                    logits[r, at] = 9.0 + torch.rand(k, generator=g) * 4.0
+                u = torch.rand(24, generator=g)
+                for kw in ({"top_k": k}, {"top_k": k, "temperature": 6.0},
+                           {"top_k": k, "temperature": 6.0, "min_p": 0.6}):
+                    both(cuda, logits.to(dtype), u, **kw)
+
+
 def test_cuts_of_every_size(cuda):
     """top-k from one token to the whole vocabulary, beside nuclei from nothing to everything: cuts
     from piece maxima, from bins, and past both lists; masked rows with fewer tokens than top-k."""
