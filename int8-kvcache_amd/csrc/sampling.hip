@@ -300,6 +300,12 @@ __device__ __forceinline__ bool needs_bins(const SampleArgs& a, const Params& q)
   return a.parts > 0 && !q.greedy && q.k == 0 && q.p < 1.0;
 }
 
+// Rows with a long top-k: where those passes run, their list is gathered there too.
+constexpr int kLongList = 256;
+__device__ __forceinline__ bool needs_list(const SampleArgs& a, const Params& q) {
+  return a.parts > 0 && !q.greedy && q.k > kLongList && q.k <= kList;
+}
+
 // Tokens waiting for their weights, so that those are computed by whole waves: value and index.
 constexpr int kQueue = 4096;
 struct Queue {
@@ -336,8 +342,8 @@ __global__ __launch_bounds__(kChunkThreads) void chunk_kernel(SampleArgs a) {
     for (int32_t b = run * kChunkThreads + (int32_t)threadIdx.x; b < kBins; b += a.runs * kChunkThreads) {
       a.bin_mass[r * kBins + b] = 0;
     }
-    if (run == 0 && threadIdx.x == 0) a.list_count[r] = 0;
   }
+  if (run == 0 && threadIdx.x == 0) a.list_count[r] = 0;
   // Rows whose whole mass is needed: without a filter, and with a nucleus cut alone.
   const bool summed = !q.greedy && q.k == 0 && (q.p < 1.0 ? a.parts > 0 : !(q.m > 0.0));
   for (int32_t c = c0; c < c1; ++c) {
@@ -469,12 +475,13 @@ struct Tiles {
 // Reads the tiles visit[0 .. visits), four slots per thread at a time and the next four in flight,
 // and calls token(value, index) for every token that is at least `from` (not -inf), by whole waves: what a
 // round finds is queued first.  One workgroup; queue.length is 0 before and after.
-template <int DT, typename Token>
+template <int DT, typename Token, typename Whole>
 __device__ __forceinline__ void read_tiles(const Row<DT>& row, const Tiles<DT>& tiles,
                                            const int32_t* visit, int32_t visits, float from,
-                                           Queue& queue, Token token) {
+                                           Queue& queue, Token token, Whole whole) {
   constexpr int kE = Row<DT>::kE;
   constexpr int kTogether = 4;
+  constexpr uint32_t kDense = 64 * kTogether * kE / 4;
   const int lane = threadIdx.x & 63;
   const int32_t items = visits << tiles.shift;
   const float least = fmaxf(from, -3.4028235e38f);
@@ -500,6 +507,13 @@ __device__ __forceinline__ void read_tiles(const Row<DT>& row, const Tiles<DT>& 
 #pragma unroll
     for (int u = 0; u < kTogether; ++u)
       raw[u] = row.request(slot_of(i0 + (kTogether + u) * kThreads + (int32_t)threadIdx.x));
+    // A wave whose tokens are mostly wanted takes them as they lie.
+    if (__builtin_amdgcn_readfirstlane(last_lane(wave_scan<uint32_t>((uint32_t)__popc(hits)))) > kDense) {
+#pragma unroll
+      for (int u = 0; u < kTogether; ++u)
+        if (slot[u] >= 0) whole(v[u], (hits >> (u * kE)) & ((1u << kE) - 1), slot[u]);
+      hits = 0;
+    }
     // (Barriers that leave the requests in flight.)
     for (int32_t found = kQueue + 1; found > kQueue;) {
       const uint32_t n = (uint32_t)__popc(hits);
@@ -654,9 +668,15 @@ __global__ __launch_bounds__(kThreads) void bins_kernel(SampleArgs a) {
   __syncthreads();
   const Row<DT> row(a, r);
   const Weights w{0x1.71547652b82fep+0 / (double)q.t, (double)top, top, a.frac};
-  read_tiles(row, tiles, s.visit, s.visits, from, s.queue, [&](float v, int32_t) {
+  const auto count = [&](float v, int32_t) {
     atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[2 * bin_of(v, top) + (t & 1)]),
               (unsigned long long)w(v));
+  };
+  read_tiles(row, tiles, s.visit, s.visits, from, s.queue, count,
+             [&](const float (&v)[Row<DT>::kE], uint32_t wanted, int32_t) {
+#pragma unroll
+    for (int j = 0; j < Row<DT>::kE; ++j)
+      if (wanted & (1u << j)) count(v[j], 0);
   });
   __syncthreads();
   for (int32_t b = t; b < kBins; b += kThreads) {
@@ -1361,6 +1381,29 @@ __device__ __forceinline__ int32_t find_bin(const T* bins, T want, T* s_wave, Sh
   return bin;
 }
 
+// The bin down to which a list for top-k is gathered, from the tiles' maxima (in `counts`, zero
+// before): all bins where every live token fits the list, else for a top-k of at most half the
+// tiles that of the k-th largest maximum (at least k tokens, hardly more than twice as many), and
+// for a larger one a guess as if the tiles were random samples of the row.  -1: more than three
+// tokens per tile, where such a guess is often wrong.
+template <int DT, typename Shared>
+__device__ __forceinline__ int32_t list_bin(const Tiles<DT>& tiles, int32_t top_k, float tile_max,
+                                            float top, uint32_t* counts, Shared& s,
+                                            uint32_t* s_wave) {
+  if (tile_max > -INFINITY) atomicAdd(&counts[bin_of(tile_max, top)], 1u);
+  const uint32_t live = (uint32_t)__syncthreads_count(tile_max > -INFINITY);
+  const uint32_t k = (uint32_t)top_k;
+  if ((live << tiles.pieces_shift) <= kList / kPieceElements) return kBins - 1;
+  if (k > 3 * live) return -1;
+  uint32_t rank = k, before, all;
+  if (k > live / 2) {
+    const float share = 1.0f - expf(-1.3f * (float)k / (float)live - 0.3f);
+    rank = (uint32_t)ceilf((float)live * share);
+    rank = rank < live ? rank : live;
+  }
+  return find_bin<uint32_t>(counts, rank, s_wave, s, before, all);
+}
+
 // The bin in which a nucleus cut alone falls (`total`: the row's mass).
 template <typename Shared>
 __device__ __forceinline__ int32_t nucleus_bin(const Params& q, uint64_t total,
@@ -1382,15 +1425,17 @@ __device__ __forceinline__ float bin_from(int32_t bin, float top) {
   return (float)((double)top - (double)d) - (fabsf(top) + d) * 0x1p-20f;
 }
 
+constexpr int kTileCopies = 4;
 struct GatherShared {
   union {
     uint64_t bin_mass[kBins];
     Queue queue;  // (once the bin is found)
   };
   uint64_t place[kList];
-  uint64_t tile_mass[kMaxTiles];
+  uint64_t tile_mass[kTileCopies * kMaxTiles];
   int32_t visit[kMaxTiles];
   uint64_t wave64[kWaves];
+  uint32_t wave32[kWaves];
   float wave_max[kWaves];
   uint64_t value64[1];
   int32_t value32[7];
@@ -1406,44 +1451,76 @@ __global__ __launch_bounds__(kThreads) void gather_kernel(SampleArgs a) {
   const int32_t part = (int32_t)(blockIdx.x - r * a.parts);
   const int t = threadIdx.x;
   const Params q = row_params(a, r);
-  if (!needs_bins(a, q)) return;
+  const bool listed = needs_list(a, q);
+  if (!needs_bins(a, q) && !listed) return;
   const Tiles<DT> tiles(a);
   const int32_t per = (tiles.count + a.parts - 1) / a.parts;
   const int32_t tile0 = part * per;
   const int32_t tile1 = tile0 + per < tiles.count ? tile0 + per : tiles.count;
   if (tile0 >= tile1) return;
-  for (int32_t b = t; b < kBins; b += kThreads) s.bin_mass[b] = a.bin_mass[r * kBins + b];
+  for (int32_t b = t; b < kBins; b += kThreads) s.bin_mass[b] = listed ? 0 : a.bin_mass[r * kBins + b];
+  const float any_max = listed && t < tiles.count ? tiles.max_of(a, r, t) : -INFINITY;
   const float tile_max = t < tile1 - tile0 ? tiles.max_of(a, r, tile0 + t) : -INFINITY;
   const Chunk chunk = own_chunk(a, r);
   if (t == 0) s.visits = s.length = 0;
-  s.tile_mass[t] = 0;
+#pragma unroll
+  for (int c = 0; c < kTileCopies; ++c) s.tile_mass[c * kMaxTiles + t] = 0;
   const float top = row_max(chunk, s.wave_max);  // (with a barrier)
   if (top == -INFINITY) return;
   const Row<DT> row(a, r);
   const Weights w{0x1.71547652b82fep+0 / (double)q.t, (double)top, top, a.frac};
   const uint64_t least = least_weight(q.m, a.frac);
-  uint64_t mass, total, before, binned;
-  double factor;
-  scan_chunks(chunk, q, top, s.wave64, mass, factor, total);
-  const int32_t bin = nucleus_bin(q, total, s.bin_mass, s, before, binned);
+  // The list's bins: [least_bin, bin].
+  int32_t bin, least_bin = 0;
+  if (listed) {
+    bin = list_bin(tiles, q.k, any_max, top, reinterpret_cast<uint32_t*>(s.bin_mass), s, s.wave32);
+    if (bin < 0) return;  // (an empty list)
+    __syncthreads();
+  } else {
+    uint64_t mass, total, before, binned;
+    double factor;
+    scan_chunks(chunk, q, top, s.wave64, mass, factor, total);
+    bin = least_bin = nucleus_bin(q, total, s.bin_mass, s, before, binned);
+  }
   const float from = bin_from(bin, top);
   if (t == 0) s.queue.length = 0;
   if (tile_max >= from && tile_max > -INFINITY) s.visit[atomicAdd(&s.visits, 1)] = tile0 + t;
   __syncthreads();
-  read_tiles(row, tiles, s.visit, s.visits, from, s.queue, [&](float v, int32_t index) {
+  // The mass that a token adds to its tile, or its place in the list.
+  const auto take = [&](float v, int32_t index) {
     const int32_t b = bin_of(v, top);
-    if (b < bin) {
+    if (b < least_bin) {
       const uint64_t x = w(v);
-      if (x >= least && x > 0)
-        atomicAdd(reinterpret_cast<unsigned long long*>(&s.tile_mass[tiles.of(row, index) - tile0]),
-                  (unsigned long long)x);
-    } else if (b == bin) {
+      return x >= least ? x : (uint64_t)0;
+    }
+    if (b <= bin) {
       const int32_t at = atomicAdd(&s.length, 1);
       if (at < kList) s.place[at] = place_of(key_of(v), index);
     }
+    return (uint64_t)0;
+  };
+  const auto add = [&](int32_t tile, uint64_t x) {
+    if (x > 0)
+      atomicAdd(reinterpret_cast<unsigned long long*>(
+                    &s.tile_mass[kTileCopies * (tile - tile0) + (t & (kTileCopies - 1))]),
+                (unsigned long long)x);
+  };
+  read_tiles(row, tiles, s.visit, s.visits, from, s.queue,
+             [&](float v, int32_t index) { add(tiles.of(row, index), take(v, index)); },
+             [&](const float (&v)[Row<DT>::kE], uint32_t wanted, int32_t slot) {
+    uint64_t sum = 0;
+#pragma unroll
+    for (int j = 0; j < Row<DT>::kE; ++j)
+      if (wanted & (1u << j)) sum += take(v[j], row.first(slot) + j);
+    add(slot >> tiles.shift, sum);
   });
   __syncthreads();
-  if (t < tile1 - tile0) a.tile_mass[r * kMaxTiles + tile0 + t] = s.tile_mass[t];
+  if (t < tile1 - tile0) {
+    uint64_t m = 0;
+#pragma unroll
+    for (int c = 0; c < kTileCopies; ++c) m += s.tile_mass[kTileCopies * t + c];
+    a.tile_mass[r * kMaxTiles + tile0 + t] = m;
+  }
   const int32_t n = s.length;
   if (t == 0) s.value32[6] = n > 0 ? atomicAdd(&a.list_count[r], n) : 0;
   __syncthreads();
@@ -1469,6 +1546,7 @@ __global__ __launch_bounds__(kThreads) void row_kernel(SampleArgs a) {
   const Tiles<DT> tiles(a);
   const bool filter = q.k > 0 || q.p < 1.0;
   const bool counted = needs_bins(a, q);  // histogram and list are there
+  const bool listed = needs_list(a, q);   // a list is
   const float tile_max = t < tiles.count ? tiles.max_of(a, r, t) : -INFINITY;
   const Chunk chunk = own_chunk(a, r);
   s.tile_mass[t] = counted && t < tiles.count ? a.tile_mass[r * kMaxTiles + t] : 0;
@@ -1480,7 +1558,7 @@ __global__ __launch_bounds__(kThreads) void row_kernel(SampleArgs a) {
         s.list.bin_count[b] = 0;
     }
   if (t == 0) {
-    s.length = counted ? a.list_count[r] : 0;
+    s.length = counted || listed ? a.list_count[r] : 0;
     s.visits = s.queue.length = 0;
     s.value32[4] = kMaxTiles;  // first tile with the maximum
   }
@@ -1522,22 +1600,19 @@ __global__ __launch_bounds__(kThreads) void row_kernel(SampleArgs a) {
   } else {
     int32_t last = kBins - 1;
     bool counting = false;
-    if (filter) {
-      if (tile_max > -INFINITY) atomicAdd(&s.list.bin_count[bin_of(tile_max, top)], 1u);
-      const uint32_t live = (uint32_t)__syncthreads_count(tile_max > -INFINITY);
-      // All live tokens fit the list?  Else down to the bin of the `rank`-th largest maximum.
-      if ((live << tiles.pieces_shift) > kList / kPieceElements) {
-        const uint32_t k = (uint32_t)(q.k > 0 ? q.k : a.vocab);
-        uint32_t rank = k, before, all;
-        if (k > live / 2) {
-          const float share = 1.0f - expf(-1.3f * (float)k / (float)live - 0.3f);
-          rank = (uint32_t)ceilf((float)live * share);
-          rank = rank < live ? rank : live;
-        }
-        confirmed = k <= kList;  // (no list could hold it)
-        counting = k > 3 * live;
-        if (!counting) last = find_bin<uint32_t>(s.list.bin_count, rank, s.wave32, s, before, all);
-      }
+    bool done = false;
+    if (listed) {
+      const int32_t n = s.length;
+      done = n >= q.k && n <= kList;
+      counting = !done;
+      for (int32_t i = t; i < n && done; i += kThreads) s.list.place[i] = a.list[r * kList + i];
+      __syncthreads();
+      if (t == 0 && !done) s.length = 0;
+    } else if (filter) {
+      confirmed = q.k <= kList;  // (no list could hold it)
+      if (confirmed) last = list_bin(tiles, q.k > 0 ? q.k : kList, tile_max, top, s.list.bin_count, s, s.wave32);
+      counting = last < 0;
+      last = counting ? kBins - 1 : last;
     } else {
       // min-p alone: w >= m is M - v <= -T ln m (and a little more, for the roundings).
       const double d = -log(q.m) * (double)q.t * (1.0 + 0x1p-20) + 0x1p-100;
@@ -1545,7 +1620,7 @@ __global__ __launch_bounds__(kThreads) void row_kernel(SampleArgs a) {
     }
     // A guess that was too high or too low is followed by a count of the row's tokens per bin, and
     // that by the list down to the bin of the k-th.
-    for (int turn = counting ? 1 : 0; confirmed; ++turn) {
+    for (int turn = counting ? 1 : 0; confirmed && !done; ++turn) {
       if (counting) {
         __syncthreads();
         for (int32_t b = t; b < kBins; b += kThreads) s.list.bin_count[b] = 0;
