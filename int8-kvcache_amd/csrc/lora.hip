@@ -9,6 +9,12 @@
 // the upper bits and the rest (together 17 bits, of a rank-wide vector), so that both products run
 // on bf16 matrix instructions and the result differs from an fp32 one by less than its own
 // rounding to bf16 does.
+//
+// Bound: for few tokens by the adapters' bytes and two launches (one token, 3584 x 4608, rank 16:
+// 7.5 us, where a launch that exits at once takes 2 to 3; 1100 tokens on 16 adapters, 18944 x 3584,
+// rank 32: 25.3 us, whose bytes alone take 14.4 at a copy's rate); for many by reading the base and
+// writing the result (6007 tokens, 3584 x 37888: 229 us, of them 214 in the second product at
+// 4.3 TB/s).
 
 #include <hip/hip_runtime.h>
 

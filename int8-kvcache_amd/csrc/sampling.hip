@@ -7,9 +7,17 @@
 // at tau.  The token is then the inverse of the cumulative kept weight in index order.
 //
 // Which token comes out depends on sums over the whole vocabulary, next to borders that a
-// rounding could move, so weights are exact to about 2^-44: 2^y by a polynomial in 64 bits (the
-// vector rate of 64-bit multiply-adds is that of 32-bit ones), rounded to a fixed-point integer.
+// rounding could move, so weights are exact to about 2^-41 (2^-44 at 152064 tokens): 2^y by a
+// polynomial in 64 bits, rounded to a fixed-point integer.
 // Integer sums do not depend on their order: chunking and atomics cannot change a result.
+//
+// Launches: chunk_kernel reads the logits once (maxima, and masses where the row needs its whole
+// one); bins_kernel and gather_kernel, where some row may have a nucleus cut over a long row, find
+// its bin and the tokens in it; row_kernel finishes a row.  What bounds them: the first pass by
+// memory where no mass is needed (37 MB of 61 x 152064 fp32: 9.0 us, 4.1 TB/s) and by 64-bit
+// arithmetic where it is (156 MB of 256 x 152064 fp32: 43.5 us, 3.6 TB/s; a copy of that size reads
+// and writes 5 TB/s); the others by the latency of their steps, each a load, a barrier or a scan of
+// one workgroup that waits for the one before (about 1 us each).
 
 #include <hip/hip_runtime.h>
 
@@ -157,6 +165,8 @@ __device__ __forceinline__ double exp2_scale(int32_t n, int32_t frac) {
 constexpr double kRound = 0x1.8p52;  // y + kRound - kRound: y rounded to an integer, left in the low bits
 
 // Rounded to integers by adding 2^52: the integer is left in the low bits.
+//
+// 19 operations of 64 bits, each 8 cycles of a wave where 32-bit ones take 4.
 struct Weights {
   double c;    // log2(e) / T
   double top;  // M
@@ -300,7 +310,10 @@ __device__ __forceinline__ bool needs_bins(const SampleArgs& a, const Params& q)
   return a.parts > 0 && !q.greedy && q.k == 0 && q.p < 1.0;
 }
 
-// Rows with a long top-k: where those passes run, their list is gathered there too.
+// Rows with a long top-k: where those passes run, their list is gathered there too, since one
+// workgroup reads a long row's tiles slowly.  (61 x 152064 fp32 beside rows with a nucleus cut:
+// top-k 256 takes 23.0 us in row_kernel, 257 takes 11.4 there and 16.4 in gather_kernel, where the
+// other rows' parts hide it; 1000 took 37.5 and takes 13.4 and 23.3.)
 constexpr int kLongList = 256;
 __device__ __forceinline__ bool needs_list(const SampleArgs& a, const Params& q) {
   return a.parts > 0 && !q.greedy && q.k > kLongList && q.k <= kList;
@@ -318,7 +331,8 @@ struct Queue {
 // A run of chunks of one row, each held in registers while the next one is loaded: the maxima of
 // their pieces and their own, and, for rows whose whole mass is needed, the sum of their weights in
 // units of their own maximum (so that the data is read once).  Clears the row's bins where they
-// will be used.
+// will be used.  Workgroups of four waves: four share a compute unit (106 registers a lane),
+// so that one reads while another computes.
 template <int DT>
 __global__ __launch_bounds__(kChunkThreads) void chunk_kernel(SampleArgs a) {
   constexpr int kE = Row<DT>::kE;
@@ -473,15 +487,19 @@ struct Tiles {
 };
 
 // Reads the tiles visit[0 .. visits), four slots per thread at a time and the next four in flight,
-// and calls token(value, index) for every token that is at least `from` (not -inf), by whole waves: what a
-// round finds is queued first.  One workgroup; queue.length is 0 before and after.
+// and calls token(value, index) for every token that is at least `from` (not -inf), by whole waves:
+// what a round finds is queued first.  A wave that wants at least half of its values calls
+// whole(values, mask, slot) for its slots instead: a queue of 4096 takes a workgroup's 32768 values
+// in eight turns (274 x 32000 bf16, nearly flat: the histogram pass 34 us, with the queue alone 61;
+// 200 x 50257 with few tokens wanted: 23 us either way, 25 where a quarter is enough).  One
+// workgroup; queue.length is 0 before and after.
 template <int DT, typename Token, typename Whole>
 __device__ __forceinline__ void read_tiles(const Row<DT>& row, const Tiles<DT>& tiles,
                                            const int32_t* visit, int32_t visits, float from,
                                            Queue& queue, Token token, Whole whole) {
   constexpr int kE = Row<DT>::kE;
   constexpr int kTogether = 4;
-  constexpr uint32_t kDense = 64 * kTogether * kE / 4;
+  constexpr uint32_t kDense = 64 * kTogether * kE / 2;
   const int lane = threadIdx.x & 63;
   const int32_t items = visits << tiles.shift;
   const float least = fmaxf(from, -3.4028235e38f);
@@ -507,7 +525,6 @@ __device__ __forceinline__ void read_tiles(const Row<DT>& row, const Tiles<DT>& 
 #pragma unroll
     for (int u = 0; u < kTogether; ++u)
       raw[u] = row.request(slot_of(i0 + (kTogether + u) * kThreads + (int32_t)threadIdx.x));
-    // A wave whose tokens are mostly wanted takes them as they lie.
     if (__builtin_amdgcn_readfirstlane(last_lane(wave_scan<uint32_t>((uint32_t)__popc(hits)))) > kDense) {
 #pragma unroll
       for (int u = 0; u < kTogether; ++u)
@@ -624,7 +641,7 @@ __device__ __forceinline__ void read_tiles_sparse(const Row<DT>& row, const Tile
 // row's (integers: in any order).  Tokens with w < (1 - p) Z / vocab cannot be kept (they and all
 // behind them weigh less than (1 - p) Z together) and are left out.  Two copies of the histogram
 // lie interleaved, a lane's copy by its number: most tokens fall into about a hundred bins, and
-// lanes that meet on one address go one after the other.
+// lanes that meet on one address go one after the other (four copies: no faster).
 struct PartShared {
   Queue queue;
   uint64_t mass[2 * kBins];
@@ -1443,7 +1460,9 @@ struct GatherShared {
 };
 
 // One part of the tiles of a row with a nucleus cut alone, its histogram finished: the tokens of
-// the bin where the cut falls, and the mass of those before it per tile.
+// the bin where the cut falls, and the mass of those before it per tile (four copies, a lane's by
+// its number: neighbours share a tile).  For rows with a long top-k, the tokens of all bins down to
+// the list's.
 template <int DT>
 __global__ __launch_bounds__(kThreads) void gather_kernel(SampleArgs a) {
   __shared__ GatherShared s;
@@ -1530,12 +1549,14 @@ __global__ __launch_bounds__(kThreads) void gather_kernel(SampleArgs a) {
 }
 
 // One row.  Rows without a filter need the chunks' masses only.  Otherwise the cut lies in a list
-// of tokens that are put in exact order: with a nucleus cut alone those that gather_kernel left,
-// else all tokens down to a logit that the piece maxima give.  For a top-k of at most half the
-// pieces that is the k-th largest of them (at least k tokens, hardly more than twice as many); for
-// a larger one a guess, as if the pieces were random samples of the row, which the list's length
-// then confirms or not.  Tiles whose maximum shows that they hold no token of the list or before
-// it are not read.
+// of tokens that are put in exact order: the one that gather_kernel left, else all tokens down to
+// the bin that list_bin gives.  Where that bin was too high or too low, the row's tokens are counted
+// per bin, which gives it exactly (32 x 50257 fp32, top-k 1000: 28.6 us; by the digits 88).  Tiles
+// whose maximum shows that they hold no token of the list or before it are not read.
+//
+// Bound by its steps' latency: 32 x 152064 bf16 with all filters 14.7 us, of those 1.7 for the
+// maximum, 1.7 for the bin, 4 for reading 50 tiles, 2.6 for the order and cut and 2 for the choice;
+// a row without a filter 6.
 template <int DT>
 __global__ __launch_bounds__(kThreads) void row_kernel(SampleArgs a) {
   __shared__ RowShared s;
