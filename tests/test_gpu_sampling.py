@@ -162,6 +162,22 @@ def test_cuts_of_every_size(cuda):
             both(cuda, logits, u, top_k=ks)  # (without top_p no histogram pass runs)
 
 
+def test_long_top_k_beside_nuclei(cuda):
+    """Rows with a long top-k in a batch where others have a nucleus cut alone, of any spread: their
+    lists are gathered beside the others' histograms."""
+    g = torch.Generator().manual_seed(16)
+    ks = [257, 300, 590, 1000, 1700, 4096, 0, 0, 257, 1500]
+    for vocab in (50257, 152064, 300007):
+        for dtype in DTYPES:
+            logits = torch.randn(len(ks), vocab, generator=g) * \
+                torch.tensor([3.0, 1.0, 0.1, 3.0, 8.0, 3.0, 0.3, 3.0, 3.0, 3.0])[:, None]
+            logits[8, torch.rand(vocab, generator=g) < 0.999] = -INF  # (fewer than k in all)
+            logits[9, vocab // 8:] = -INF
+            u = torch.rand(len(ks), generator=g)
+            for kw in ({"top_p": 0.9}, {"top_p": 0.97, "min_p": 0.01, "temperature": 1.4}):
+                both(cuda, logits.to(dtype), u, top_k=ks, **kw)
+
+
 def test_live_tokens_in_few_places(cuda):
     """All live tokens in one corner of the row, more and fewer than the list holds."""
     g = torch.Generator().manual_seed(15)
