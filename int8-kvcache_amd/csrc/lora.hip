@@ -3,7 +3,8 @@
 //
 // A plan groups the tokens by adapter into tiles of one adapter each (16 tokens, or 64 in larger
 // batches); the products then run tile by tile on matrix instructions, in two launches: x A^T into
-// fp32 partial sums (split along k), then those times B^T, the scale and the base.
+// fp32 partial sums (split along k), then those times B^T, the scale and the base; or in one, where
+// A is small.
 //
 // Precision: the first product's sums stay fp32.  They enter the second one as two bf16 parts,
 // the upper bits and the rest (together 17 bits, of a rank-wide vector), so that both products run
@@ -308,6 +309,27 @@ __global__ __launch_bounds__(kShrinkWaves<TT> * 64) void shrink_kernel(LoraArgs 
       }
 }
 
+// Rank r's value of a token as two bf16 parts: upper (truncated: no overflow) and rest.
+__device__ __forceinline__ void stage_value(uint16_t* row, int32_t r, int32_t rank, float h) {
+  const uint32_t hi = __float_as_uint(h) >> 16;
+  row[r] = (uint16_t)hi;
+  row[rank + r] = fabsf(h) < INFINITY ? (uint16_t)bf16_bits(h - bf16_value(hi)) : 0;
+}
+
+// Eight columns: bf16(base + scale * products).
+__device__ __forceinline__ u32x4 add_scaled(const float* product, float scale, u32x4 base) {
+  const f32x4 d[2] = {*reinterpret_cast<const f32x4*>(product),
+                      *reinterpret_cast<const f32x4*>(product + 4)};
+  u32x4 o;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float lo = d[j >> 1][2 * (j & 1)] * scale + bf16_value(base[j] & 0xffffu);
+    const float hi = d[j >> 1][2 * (j & 1) + 1] * scale + bf16_value(base[j] >> 16);
+    o[j] = bf16_bits(lo) | (bf16_bits(hi) << 16);
+  }
+  return o;
+}
+
 // The second product of one tile and one chunk of columns.  The rank-wide vectors are staged in
 // LDS as two bf16 parts, upper (truncated: no overflow) and rest; along the product's inner axis
 // first all upper parts, then all rests, against the same row of B.  NS: 32-wide steps of that
@@ -431,12 +453,7 @@ __global__ __launch_bounds__(kExpandWaves * 64) void expand_kernel(LoraArgs a) {
     const int32_t r = p / quads;
     const int32_t c = 4 * (p - r * quads);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t hi = __float_as_uint(h[j]) >> 16;
-      const float rest = h[j] - bf16_value(hi);
-      s_h[r][c + j] = (uint16_t)hi;
-      s_h[r][a.rank + c + j] = fabsf(h[j]) < INFINITY ? (uint16_t)bf16_bits(rest) : 0;
-    }
+    for (int j = 0; j < 4; ++j) stage_value(&s_h[r][0], c + j, a.rank, h[j]);
   };
   for (int32_t p = p0; p < kRows * quads; p += kExpandWaves * 64) {
     f32x4 h = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -491,20 +508,145 @@ __global__ __launch_bounds__(kExpandWaves * 64) void expand_kernel(LoraArgs a) {
       for (int j = 0; j < 4; ++j) *reinterpret_cast<f32x4*>(&s_out[wave][i][16 * j + 4 * g]) = acc[j];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float* q = &s_out[wave][8 * h + line][8 * (lane & 7)];
-        const f32x4 d[2] = {*reinterpret_cast<const f32x4*>(q), *reinterpret_cast<const f32x4*>(q + 4)};
-        u32x4 o;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float lo = d[j >> 1][2 * (j & 1)] * scale + bf16_value(v[h][j] & 0xffffu);
-          const float hi = d[j >> 1][2 * (j & 1) + 1] * scale + bf16_value(v[h][j] >> 16);
-          o[j] = bf16_bits(lo) | (bf16_bits(hi) << 16);
-        }
+        const u32x4 o = add_scaled(&s_out[wave][8 * h + line][8 * (lane & 7)], scale, v[h]);
         if (in_here && 16 * tt + 8 * h + line < rows)
           store16<STREAM>(a.out + (int64_t)token[tt][h] * a.out_stride + here, o);
       }
     }
   }
+}
+
+// Both products of one tile of 16 tokens and 512 columns, for adapters whose A is small: every
+// workgroup forms the tile's x A^T itself (its waves take the 32-wide steps of k in turn and add up
+// through LDS), which saves the first product's launch and the partial sums' way through memory.
+// B and the base rows are requested before the first product.  Bound by one launch's chain of loads
+// (plan, then x, A, B and base) and by the rate at which a compute unit loads A.  One token, 1024 x
+// 4096, rank 8: 4.2 us.
+constexpr int kBothWaves = 8;
+constexpr int kBothColumns = kBothWaves * kWaveColumns;
+template <int RT, int NS, bool PAIRED>
+__global__ __launch_bounds__(kBothWaves * 64) void both_kernel(LoraArgs a) {
+  constexpr int kHeld = PAIRED ? NS / 2 : NS;
+  constexpr int kFlight = RT == 1 ? 8 : 6;
+  constexpr int kStep = 32 * kBothWaves;
+  __shared__ __align__(16) uint16_t s_h[16][32 * NS + 8];
+  __shared__ union {
+    f32x4 acc[kBothWaves][RT * 64];
+    float out[kBothWaves][16][kWaveColumns + 4];
+  } s;
+  const int32_t tile = blockIdx.x / a.groups;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int i = lane & 15;
+  const int g = lane >> 4;
+  const int line = lane >> 3;
+  const int2 head = a.plan.head[tile];
+  const int32_t mine = a.plan.token[tile * 16 + i];
+  int32_t token[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) token[h] = a.plan.token[tile * 16 + 8 * h + line];
+  const int32_t adapter = __builtin_amdgcn_readfirstlane(head.x);
+  const int32_t rows = __builtin_amdgcn_readfirstlane(head.y);
+  if (rows == 0) return;
+  const int32_t first = __builtin_amdgcn_readlane(mine, 0);
+  const int32_t col0 = (int32_t)(blockIdx.x - tile * a.groups) * kBothColumns + wave * kWaveColumns;
+  const int32_t col = col0 + 8 * (lane & 7);
+  const bool in = col < a.n;
+  u32x4 base[2];
+  const auto request_base = [&]() {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int64_t t = 8 * h + line < rows ? token[h] : first;
+      base[h] = load16<false>(a.base + t * a.base_stride + (in ? col : 0));
+    }
+  };
+  const auto store = [&](int h, u32x4 v) {
+    if (in && 8 * h + line < rows)
+      store16<false>(a.out + (int64_t)token[h] * a.out_stride + col, v);
+  };
+  if (adapter < 0) {
+    if (a.out == a.base && a.out_stride == a.base_stride) return;
+    request_base();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) store(h, base[h]);
+    return;
+  }
+  const uint16_t* xp = a.x + (int64_t)(i < rows ? mine : first) * a.x_stride + 8 * g;
+  const uint16_t* ap[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int32_t r = 16 * rt + i;
+    ap[rt] = a.a + adapter * a.a_adapter + (int64_t)(r < a.rank ? r : a.rank - 1) * a.a_row + 8 * g;
+  }
+  f32x4 acc[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) acc[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  bf16x8 xv[kFlight], av[kFlight][RT];
+  const auto request = [&](int f, int32_t k) {
+    const bool inside = k + 8 * g < a.k;  // k is a multiple of 8
+    xv[f] = inside ? load8(xp + k) : zero8();
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) av[f][rt] = inside ? load8(ap[rt] + k) : zero8();
+  };
+  int32_t k = 32 * wave;
+#pragma unroll
+  for (int f = 0; f < kFlight; ++f) request(f, k + f * kStep);
+  const int32_t granules = a.rank / 8;
+  bf16x8 bv[kHeld][4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int32_t c = col0 + 16 * j + i;
+    const uint16_t* bp = a.b + adapter * a.b_adapter + (int64_t)(c < a.n ? c : a.n - 1) * a.b_row;
+#pragma unroll
+    for (int t = 0; t < kHeld; ++t) {
+      const int32_t p = 4 * t + g;
+      bv[t][j] = p < 2 * granules ? load8(bp + 8 * (p < granules ? p : p - granules)) : zero8();
+    }
+  }
+  request_base();
+  const float scale = a.scales ? a.scales[adapter] : 1.0f;
+  for (; k < a.k; k += kFlight * kStep) {
+#pragma unroll
+    for (int f = 0; f < kFlight; ++f) {
+      const bf16x8 x = xv[f];
+      bf16x8 w[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) w[rt] = av[f][rt];
+      request(f, k + (kFlight + f) * kStep);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+        acc[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[rt], x, acc[rt], 0, 0, 0);
+    }
+  }
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) s.acc[wave][rt * 64 + lane] = acc[rt];
+  __syncthreads();
+  // Value v of the tile: of rank 16 rt + 4 g + c and token i, v = 4 (64 rt + 16 g + i) + c.
+  for (int32_t v = threadIdx.x; v < RT * 256; v += kBothWaves * 64) {
+    float h = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kBothWaves; ++w) h += reinterpret_cast<const float*>(s.acc[w])[v];
+    const int32_t r = 16 * (v >> 8) + 4 * ((v >> 6) & 3) + (v & 3);
+    if (r < a.rank) stage_value(&s_h[(v >> 2) & 15][0], r, a.rank, h);
+  }
+  __syncthreads();
+  f32x4 sum[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) sum[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int t = 0; t < NS; ++t) {
+    const int32_t p = 4 * t + g;
+    const bf16x8 hv = p < 2 * granules ? load8(&s_h[i][8 * p]) : zero8();
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      sum[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(bv[t % kHeld][j], hv, sum[j], 0, 0, 0);
+  }
+  // (The wave's own buffer.)
+#pragma unroll
+  for (int j = 0; j < 4; ++j) *reinterpret_cast<f32x4*>(&s.out[wave][i][16 * j + 4 * g]) = sum[j];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    store(h, add_scaled(&s.out[wave][8 * h + line][8 * (lane & 7)], scale, base[h]));
 }
 
 bool rows16(const void* p, int64_t stride) {
@@ -526,6 +668,18 @@ int splits_for(int64_t tiles, int64_t k, int rows) {
   return (int)(s < 1 ? 1 : (s < 16 ? s : 16));
 }
 
+// Both products in one launch?  A launch costs about 2.5 us and one compute unit loads A at about
+// 30 bytes a ns, so where an adapter's A has at most 64 KB, and all workgroups' together 64 KB per
+// compute unit (one token: 1024 x 4096, rank 8: 6.6 us in two launches, 4.2 in one; 2048 x 4608,
+// rank 16: 6.5 and 5.6; 3584 x 4608, 112 KB: 6.5 and 7.2; 100 tokens on 40 adapters, 1024 x 4096,
+// rank 16: 7.9 and 6.5; 250, 2048 x 4608: 8.4 and 10.6).
+bool both_at_once(int64_t tiles, int rows, int64_t k, int32_t rank, int64_t n) {
+  constexpr int64_t kMost = 64 << 10, kUnits = 256;
+  const int64_t bytes = 2 * rank * k;
+  return rows == 16 && rank <= 32 && bytes <= kMost &&
+         tiles * ((n + kBothColumns - 1) / kBothColumns) * bytes <= kMost * kUnits;
+}
+
 bool lora_sizes_ok(int64_t tokens, int32_t adapters, int64_t k, int32_t rank) {
   return tokens >= 0 && tokens <= kMaxTokens && adapters >= 1 && adapters <= kMaxAdapters &&
          k >= 8 && k % 8 == 0 && k <= kMaxWidth && rank >= 8 && rank % 8 == 0 && rank <= kMaxRank;
@@ -540,6 +694,24 @@ void launch_shrink(const LoraArgs& a, hipStream_t s) {
     hipLaunchKernelGGL((shrink_kernel<TT, 2>), grid, block, 0, s, a);
   else
     hipLaunchKernelGGL((shrink_kernel<TT, 4>), grid, block, 0, s, a);
+}
+
+void launch_both(const LoraArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)(a.plan.tiles * a.groups)), block(kBothWaves * 64);
+  const bool paired = a.rank % 32 == 0;
+  switch ((2 * a.rank + 31) / 32) {
+#define INT8KV_BOTH(RT, NS, PAIRED) \
+  hipLaunchKernelGGL((both_kernel<RT, NS, PAIRED>), grid, block, 0, s, a)
+    case 1: INT8KV_BOTH(1, 1, false); break;
+    case 2:
+      if (paired)
+        INT8KV_BOTH(2, 2, true);
+      else
+        INT8KV_BOTH(2, 2, false);
+      break;
+#undef INT8KV_BOTH
+    default: break;
+  }
 }
 
 template <int TT, bool STREAM>
@@ -668,6 +840,12 @@ extern "C" int int8kv_lora_add(const void* base, int64_t base_row_stride, const 
   a.rank = rank;
   const int64_t tiles = a.plan.tiles;
   const int rows = tile_rows(tokens, num_adapters);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (both_at_once(tiles, rows, k, rank, n)) {
+    a.groups = (int32_t)((n + kBothColumns - 1) / kBothColumns);
+    launch_both(a, s);
+    return (int)hipGetLastError();
+  }
   a.splits = splits_for(tiles, k, rows);
   a.chunk = (int32_t)(((k + a.splits - 1) / a.splits + 31) / 32 * 32);
   a.halves = (rank + 63) / 64;
@@ -678,7 +856,6 @@ extern "C" int int8kv_lora_add(const void* base, int64_t base_row_stride, const 
   a.run = (int32_t)(run < 1 ? 1 : (run < 8 ? run : 8));
   a.groups = (a.chunks + a.run - 1) / a.run;
   if (tiles * (a.groups + kXcds) > 0x7fffffff) return INT8KV_E_SHAPE;
-  hipStream_t s = static_cast<hipStream_t>(stream);
   if (rows == 64) {
     launch_shrink<4>(a, s);
     if (4 * tokens * n > kInfinityCacheBytes)

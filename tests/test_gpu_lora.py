@@ -196,3 +196,30 @@ def test_misaligned_rows_are_refused(cuda):
         int8kv.lora_add(d["base"], wide[:, 1:65], d["a"], d["b"], plan)
     with pytest.raises(AssertionError):
         int8kv.lora_add(d["base"][:, ::2], d["x"], d["a"], d["b"], plan)
+
+
+@pytest.mark.parametrize("tokens,k,n,rank,adapters", [
+    (20, 520, 328, 32, 9),      # one launch, rank a multiple of 32
+    (23, 1024, 264, 32, 12),    # the longest A that one launch takes
+    (40, 1024, 1544, 16, 24),
+    (300, 264, 520, 8, 48),
+    (9, 4104, 264, 24, 3),      # two launches
+    (6, 4104, 1032, 8, 4),      # a little over the longest A
+    (70, 2056, 264, 32, 30),
+])
+def test_small_tiles_of_both_forms(cuda, tokens, k, n, rank, adapters):
+    """Tiles of 16 tokens with short and with long adapters: values, infinities in their own row,
+    rows without an adapter, and out in place."""
+    d = inputs(cuda, tokens, k, n, rank, adapters, seed=tokens + rank)
+    want = add(d)
+    check(d, want)
+    none = (d["ids"] < 0) | (d["ids"] >= adapters)
+    marked = int(torch.nonzero(~none)[0])
+    d["base"][none] = float("nan")
+    d["x"][none] = float("inf")
+    d["x"][marked, k - 1] = float("-inf")
+    out = add(d, out=d["base"])
+    assert out.data_ptr() == d["base"].data_ptr() and torch.isnan(out[none]).all()
+    same = ~none
+    same[marked] = False
+    assert torch.equal(out[same], want[same]) and not torch.isfinite(out[marked]).any()
