@@ -177,6 +177,7 @@ struct LoraArgs {
   uint16_t* out;
   int64_t out_stride;
   float* part;  // [splits][tiles x rows of a tile][rank]
+  uint16_t* staged;  // [tiles x rows of a tile][2][rank]: their sums in two parts, or null
   Plan plan;
   int32_t k, n, rank;
   int32_t splits;  // parts of k
@@ -330,6 +331,32 @@ __device__ __forceinline__ u32x4 add_scaled(const float* product, float scale, u
   return o;
 }
 
+// The parts' sums, once, where many workgroups of the second product would each add them up; left
+// as the two bf16 parts (what lies behind a tile's rows or was not written: any bits, which reach
+// no row of a result).  Bound by latency: 2 to 4 us.
+constexpr int kSumThreads = 256;
+__global__ __launch_bounds__(kSumThreads) void sum_kernel(LoraArgs a, int32_t rows) {
+  constexpr int kTogether = 8;
+  const int32_t quads = a.rank / 4;
+  const int64_t q = (int64_t)blockIdx.x * kSumThreads + threadIdx.x;
+  const int64_t all = (int64_t)a.plan.tiles * rows * quads;
+  if (q >= all) return;
+  const f32x4* part = reinterpret_cast<const f32x4*>(a.part);
+  f32x4 h = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int32_t s0 = 0; s0 < a.splits; s0 += kTogether) {
+    f32x4 y[kTogether];
+#pragma unroll
+    for (int u = 0; u < kTogether; ++u) y[u] = part[(s0 + u < a.splits ? s0 + u : 0) * all + q];
+#pragma unroll
+    for (int u = 0; u < kTogether; ++u)
+      if (s0 + u < a.splits) h += y[u];
+  }
+  const int64_t row = q / quads;
+  const int32_t c = 4 * (int32_t)(q - row * quads);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) stage_value(a.staged + row * 2 * a.rank, c + j, a.rank, h[j]);
+}
+
 // The second product of one tile and one chunk of columns.  The rank-wide vectors are staged in
 // LDS as two bf16 parts, upper (truncated: no overflow) and rest; along the product's inner axis
 // first all upper parts, then all rests, against the same row of B.  NS: 32-wide steps of that
@@ -400,7 +427,19 @@ __global__ __launch_bounds__(kExpandWaves * 64) void expand_kernel(LoraArgs a) {
                                              4 * (p < kRows * quads ? p : 0));
     }
   };
-  request_parts(p0, way);
+  // Summed already: 16-byte pieces of the two parts.
+  const int32_t row_pieces = a.rank / 4;
+  const uint16_t* sums = a.staged + (int64_t)tile * kRows * 2 * a.rank;
+  const bool summed = TT > 1 && a.staged;
+  if (summed) {
+#pragma unroll
+    for (int u = 0; u < kTogether; ++u) {
+      const int32_t p = (int32_t)threadIdx.x + u * kExpandWaves * 64;
+      y[u] = *reinterpret_cast<const f32x4*>(sums + 8 * (p < kRows * row_pieces ? p : 0));
+    }
+  } else {
+    request_parts(p0, way);
+  }
   const int32_t adapter = __builtin_amdgcn_readfirstlane(head.x);
   const int32_t rows = __builtin_amdgcn_readfirstlane(head.y);
   if (rows == 0) return;
@@ -455,7 +494,16 @@ __global__ __launch_bounds__(kExpandWaves * 64) void expand_kernel(LoraArgs a) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) stage_value(&s_h[r][0], c + j, a.rank, h[j]);
   };
-  for (int32_t p = p0; p < kRows * quads; p += kExpandWaves * 64) {
+  if (summed) {
+    static_assert(TT == 1 || kRows * kMaxRank / 4 <= kTogether * kExpandWaves * 64, "one round");
+#pragma unroll
+    for (int u = 0; u < kTogether; ++u) {
+      const int32_t p = (int32_t)threadIdx.x + u * kExpandWaves * 64;
+      const int32_t r = p / row_pieces;
+      if (p < kRows * row_pieces) *reinterpret_cast<f32x4*>(&s_h[r][8 * (p - r * row_pieces)]) = y[u];
+    }
+  }
+  for (int32_t p = summed ? kRows * quads : p0; p < kRows * quads; p += kExpandWaves * 64) {
     f32x4 h = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int32_t s0 = way; s0 < a.splits; s0 += kTogether * ways) {
       if (p != p0 || s0 != way) request_parts(p, s0);
@@ -655,17 +703,22 @@ bool rows16(const void* p, int64_t stride) {
 
 // Parts of k.  Tiles of 16 tokens: about four workgroups of four waves per compute unit (32 tokens
 // on 24 adapters, the four projections of a layer: 35 us with 12-16 parts, 37 with 8, 56 with 2).
-// Tiles of 64: eight waves, about 1.5 workgroups per unit (34 tiles, 18944 x 3584: 26 us with 12
-// parts, 31 with 6, 29 with 16); from 64 tiles on no parts below 1536, since every workgroup of
-// the second product reads all parts of its tile (99 tiles, 3584 x 37888: 239 us with 2, 250 with
-// 4).  A part has at least two steps per wave.
-int splits_for(int64_t tiles, int64_t k, int rows) {
-  const int64_t shortest = rows == 16 ? 2 * 32 * kShrinkWaves<1>
-                                      : (tiles >= 64 ? 1536 : 2 * 32 * kShrinkWaves<4>);
-  const int64_t most = k / shortest;
-  int64_t s = ((rows == 16 ? 1024 : 384) + tiles - 1) / (tiles > 0 ? tiles : 1);
+// Tiles of 64: eight waves, as many workgroups as run at a time, two per unit up to rank 32 and one
+// above, where the registers leave room for no more (1100 tokens, 18944 x 3584, rank 32, 34 tiles:
+// 25.3 us with 14 parts, 27.8 with 7, 28.4 with 16; 1057 tokens, 18944 x 37888, rank 64, 20 tiles:
+// 55 with 12, 62 with 16, 64 with 6).  A part has at least two steps per wave.
+int splits_for(int64_t tiles, int64_t k, int rows, int32_t rank) {
+  const int64_t shortest = 2 * 32 * (rows == 16 ? kShrinkWaves<1> : kShrinkWaves<4>);
+  const int64_t most = k / shortest < 32 ? k / shortest : 32;
+  int64_t s;
+  if (rows == 16) {
+    s = (1024 + tiles - 1) / (tiles > 0 ? tiles : 1);
+    s = s < 16 ? s : 16;
+  } else {
+    s = (rank <= 32 ? 480 : 256) / (tiles * ((rank + 63) / 64));
+  }
   s = s < most ? s : most;
-  return (int)(s < 1 ? 1 : (s < 16 ? s : 16));
+  return (int)(s < 1 ? 1 : s);
 }
 
 // Both products in one launch?  A launch costs about 2.5 us and one compute unit loads A at about
@@ -789,7 +842,7 @@ extern "C" size_t int8kv_lora_workspace_bytes(int64_t tokens, int32_t num_adapte
   if (!lora_sizes_ok(tokens, num_adapters, k, rank)) return 0;
   const int rows = tile_rows(tokens, num_adapters);
   const int64_t tiles = max_tiles(tokens, num_adapters, rows);
-  return 16 + (size_t)tiles * rows * rank * 4 * splits_for(tiles, k, rows);
+  return 16 + (size_t)tiles * rows * rank * 4 * (splits_for(tiles, k, rows, rank) + (rows == 64 ? 1 : 0));
 }
 
 extern "C" int int8kv_lora_add(const void* base, int64_t base_row_stride, const void* x,
@@ -846,7 +899,7 @@ extern "C" int int8kv_lora_add(const void* base, int64_t base_row_stride, const 
     launch_both(a, s);
     return (int)hipGetLastError();
   }
-  a.splits = splits_for(tiles, k, rows);
+  a.splits = splits_for(tiles, k, rows, rank);
   a.chunk = (int32_t)(((k + a.splits - 1) / a.splits + 31) / 32 * 32);
   a.halves = (rank + 63) / 64;
   a.chunks = (int32_t)((n + kExpandColumns - 1) / kExpandColumns);
@@ -856,8 +909,18 @@ extern "C" int int8kv_lora_add(const void* base, int64_t base_row_stride, const 
   a.run = (int32_t)(run < 1 ? 1 : (run < 8 ? run : 8));
   a.groups = (a.chunks + a.run - 1) / a.run;
   if (tiles * (a.groups + kXcds) > 0x7fffffff) return INT8KV_E_SHAPE;
+  a.staged = nullptr;
   if (rows == 64) {
     launch_shrink<4>(a, s);
+    // The parts' sums in a launch of their own where the second product would read more than 32 MB
+    // of parts (1057 tokens, 18944 x 37888, rank 64, 776 MB: 105 us without, 64 with; 1100, 18944 x
+    // 3584, rank 32, 47 MB: 34.1 and 33.2; 523, 4096 x 4608, rank 32, 15 MB: 14.8 and 15.8).
+    if (tiles * a.groups * a.splits * rows * rank * 4 > 32 << 20) {
+      a.staged = reinterpret_cast<uint16_t*>(a.part + (int64_t)a.splits * tiles * rows * rank);
+      const int64_t quads = tiles * rows * rank / 4;
+      hipLaunchKernelGGL(sum_kernel, dim3((unsigned)((quads + kSumThreads - 1) / kSumThreads)),
+                         dim3(kSumThreads), 0, s, a, rows);
+    }
     if (4 * tokens * n > kInfinityCacheBytes)
       launch_expand<4, true>(a, s);
     else
