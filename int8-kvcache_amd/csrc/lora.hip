@@ -103,6 +103,18 @@ __device__ __forceinline__ int32_t plan_scan(int32_t v, int32_t* s_wave, int32_t
   return before + inc - v;
 }
 
+// The next place of group g (the active lanes' own).  Neighbours in a prefill share their adapter:
+// then one lane counts for all of them.
+__device__ __forceinline__ int32_t next_place(int32_t* s_count, int32_t g) {
+  const uint64_t active = __ballot(true);
+  const int32_t first = __builtin_amdgcn_readfirstlane(g);
+  if (__ballot(g == first) != active) return atomicAdd(&s_count[g], 1);
+  const int32_t before = (int32_t)__popcll(active & ((1ull << (threadIdx.x & 63)) - 1));
+  int32_t at = 0;
+  if (before == 0) at = atomicAdd(&s_count[first], (int32_t)__popcll(active));
+  return __builtin_amdgcn_readfirstlane(at) + before;
+}
+
 // One workgroup: a token's place in its group from a counter in LDS, then the groups' first tiles.
 // The order of tokens within a group may differ from call to call; no result depends on it (a
 // token's row is computed alike at every place).  HELD: all places stay in registers; otherwise
@@ -126,10 +138,10 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const void* ids, int
   if constexpr (HELD) {
 #pragma unroll
     for (int j = 0; j < kPlanTokens; ++j)
-      if (group[j] >= 0) place[j] = atomicAdd(&s_count[group[j]], 1);
+      if (group[j] >= 0) place[j] = next_place(s_count, group[j]);
   } else {
     for (int32_t t = threadIdx.x; t < tokens; t += kPlanThreads)
-      atomicAdd(&s_count[adapter_of<L64>(ids, t, adapters)], 1);
+      next_place(s_count, adapter_of<L64>(ids, t, adapters));
   }
   __syncthreads();
   // The groups' first tiles; each thread a contiguous span of groups.
@@ -158,7 +170,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const void* ids, int
   } else {
     for (int32_t t = threadIdx.x; t < tokens; t += kPlanThreads) {
       const int32_t g = adapter_of<L64>(ids, t, adapters);
-      plan.token[s_tile[g] * tile + atomicAdd(&s_count[g], 1)] = t;
+      plan.token[s_tile[g] * tile + next_place(s_count, g)] = t;
     }
   }
 }

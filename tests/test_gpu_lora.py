@@ -223,3 +223,12 @@ def test_small_tiles_of_both_forms(cuda, tokens, k, n, rank, adapters):
     same = ~none
     same[marked] = False
     assert torch.equal(out[same], want[same]) and not torch.isfinite(out[marked]).any()
+
+
+@pytest.mark.parametrize("tokens,adapters,run", [(17001, 3, 700), (20000, 4000, 1), (33000, 1, 50)])
+def test_more_tokens_than_a_plan_holds(cuda, tokens, adapters, run):
+    """Plans that count their tokens twice: runs of one adapter, and neighbours of all kinds."""
+    g = torch.Generator().manual_seed(tokens)
+    ids = torch.randint(-1, adapters, (tokens // run + 1,), generator=g).repeat_interleave(run)[:tokens]
+    d = inputs(cuda, tokens, 40, 24, 8, adapters, seed=13, ids=ids)
+    check(d, add(d))
