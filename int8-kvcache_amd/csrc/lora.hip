@@ -455,20 +455,6 @@ __global__ __launch_bounds__(kExpandWaves * 64) void expand_kernel(LoraArgs a) {
   const int32_t adapter = __builtin_amdgcn_readfirstlane(head.x);
   const int32_t rows = __builtin_amdgcn_readfirstlane(head.y);
   if (rows == 0) return;
-  if (adapter < 0) {
-    if (a.out == a.base && a.out_stride == a.base_stride) return;
-    const int32_t c0 = chunk0 * kExpandColumns;
-    const int32_t c1 = chunk1 * kExpandColumns < a.n ? chunk1 * kExpandColumns : a.n;
-    const int32_t pieces = (c1 - c0) / 8;
-    for (int32_t p = threadIdx.x; p < rows * pieces; p += kExpandWaves * 64) {
-      const int32_t r = p / pieces;
-      const int64_t t = a.plan.token[tile * kRows + r];
-      const int32_t c = c0 + 8 * (p - r * pieces);
-      *reinterpret_cast<u32x4*>(a.out + t * a.out_stride + c) =
-          *reinterpret_cast<const u32x4*>(a.base + t * a.base_stride + c);
-    }
-    return;
-  }
   const int32_t first = __builtin_amdgcn_readlane(token[0][0], 0);
   const int32_t granules = a.rank / 8;  // 8-wide pieces of one part
   int32_t col0 = chunk0 * kExpandColumns + wave * kWaveColumns;
@@ -482,6 +468,22 @@ __global__ __launch_bounds__(kExpandWaves * 64) void expand_kernel(LoraArgs a) {
       base[tt][h] = in ? load16<STREAM>(a.base + t * a.base_stride + col) : u32x4{0u, 0u, 0u, 0u};
     }
   };
+  if (adapter < 0) {
+    if (a.out == a.base && a.out_stride == a.base_stride) return;
+    for (int32_t chunk = chunk0; chunk < chunk1; ++chunk) {
+      in = col < a.n;
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt) request_base(tt);
+#pragma unroll
+      for (int tt = 0; tt < TT; ++tt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (in && 16 * tt + 8 * h + line < rows)
+            store16<STREAM>(a.out + (int64_t)token[tt][h] * a.out_stride + col, base[tt][h]);
+      col += kExpandColumns;
+    }
+    return;
+  }
 #pragma unroll
   for (int tt = 0; tt < TT; ++tt) request_base(tt);
   // Row 4 g + r of matrix tile j's operand is column 16 j + 4 g + r.
