@@ -97,14 +97,15 @@ struct Row {
   __device__ __forceinline__ int32_t first(int32_t s) const {
     return s == 0 ? 0 : head + (s - 1) * kE;
   }
-  __device__ __forceinline__ float element(int32_t i) const {
+  static __device__ __forceinline__ float value_in(const void* values, int32_t i) {
     if constexpr (DT == kF32)
-      return reinterpret_cast<const float*>(p)[i];
+      return static_cast<const float*>(values)[i];
     else if constexpr (DT == kBF16)
-      return __uint_as_float((uint32_t) reinterpret_cast<const uint16_t*>(p)[i] << 16);
+      return __uint_as_float((uint32_t) static_cast<const uint16_t*>(values)[i] << 16);
     else
-      return (float)reinterpret_cast<const _Float16*>(p)[i];
+      return (float)static_cast<const _Float16*>(values)[i];
   }
+  __device__ __forceinline__ float element(int32_t i) const { return value_in(p, i); }
   // A slot's vector, requested without a branch (an edge slot requests a neighbour's).
   __device__ __forceinline__ u32x4 request(int32_t s) const {
     const int32_t i = s - 1 < vectors - 1 ? s - 1 : vectors - 1;
@@ -631,8 +632,16 @@ __device__ __forceinline__ void read_tiles_sparse(const Row<DT>& row, const Tile
     }
   }
   __syncthreads();
+  // One value per thread.
   const int32_t n = queue.length < kSlotQueue ? queue.length : kSlotQueue;
-  for (int32_t i = threadIdx.x; i < n; i += kThreads) look(queue.slot[i], queue.raw[i]);
+  for (int32_t i = threadIdx.x; i < n * kE; i += kThreads) {
+    const int32_t slot = queue.slot[i / kE];
+    const int32_t index = row.first(slot) + i % kE;
+    const bool whole = slot >= 1 && slot <= row.vectors;
+    float v = Row<DT>::value_in(queue.raw, i);
+    if (!whole) v = index < (slot == 0 ? row.head : row.vocab) ? row.element(index) : -INFINITY;
+    if (v >= least) token(v, index);
+  }
   __syncthreads();
 }
 
