@@ -487,6 +487,17 @@ struct Tiles {
   }
 };
 
+// Adds this thread's tile to the list of those to visit, one addition per wave.
+__device__ __forceinline__ void push_visit(bool wanted, int32_t tile, int32_t* visit, int32_t* visits) {
+  const uint64_t m = __ballot(wanted);
+  if (m == 0) return;
+  const int lane = threadIdx.x & 63;
+  int32_t at = 0;
+  if (lane == 0) at = atomicAdd(visits, (int32_t)__popcll(m));
+  at = __builtin_amdgcn_readfirstlane(at) + (int32_t)__popcll(m & ((1ull << lane) - 1));
+  if (wanted) visit[at] = tile;
+}
+
 // Reads the tiles visit[0 .. visits), four slots per thread at a time and the next four in flight,
 // and calls token(value, index) for every token that is at least `from` (not -inf), by whole waves:
 // what a round finds is queued first.  A wave that wants at least half of its values calls
@@ -610,7 +621,7 @@ __device__ __forceinline__ void read_tiles_sparse(const Row<DT>& row, const Tile
       now[u] = raw[u];
       at[u] = slot[u];
     }
-    request(i0 + kTogether * kThreads);
+    if (i0 + kTogether * kThreads < items) request(i0 + kTogether * kThreads);
 #pragma unroll
     for (int u = 0; u < kTogether; ++u) {
       if (i0 + u * kThreads >= items) break;  // (uniform)
@@ -690,7 +701,7 @@ __global__ __launch_bounds__(kThreads) void bins_kernel(SampleArgs a) {
   double factor;
   scan_chunks(chunk, q, top, s.wave64, mass, factor, total);
   const float from = nucleus_from(a, q, top, total);
-  if (tile_max >= from && tile_max > -INFINITY) s.visit[atomicAdd(&s.visits, 1)] = tile;
+  push_visit(tile_max >= from && tile_max > -INFINITY, tile, s.visit, &s.visits);
   __syncthreads();
   const Row<DT> row(a, r);
   const Weights w{0x1.71547652b82fep+0 / (double)q.t, (double)top, top, a.frac};
@@ -919,27 +930,41 @@ __device__ __forceinline__ void sort_places(uint64_t (&x)[P], uint64_t* s) {
   }
 }
 
-// The order of at most kRanked places: four threads per place count the larger ones.
+// The order of at most kRanked places: four threads per place count the larger ones.  INDEXED: the
+// places' numbers by index too, left behind (index_ranks) in the order of the places.
 constexpr int kRanked = kThreads / 4;
+__device__ __forceinline__ int32_t* index_ranks(uint64_t* s) {
+  return reinterpret_cast<int32_t*>(s + 2 * kRanked) + 2 * kRanked;
+}
+template <bool INDEXED>
 __device__ __forceinline__ uint64_t rank_places(int32_t n, uint64_t* s) {
   uint64_t* sorted = s + kRanked;
   int32_t* rank = reinterpret_cast<int32_t*>(s + 2 * kRanked);
+  int32_t* by_index = rank + kRanked;
   const int t = threadIdx.x;
   const int e = t % kRanked;
-  if (t < kRanked) rank[t] = 0;
+  if (t < 2 * kRanked) rank[t] = 0;
   __syncthreads();
   const int32_t per = (n + 3) / 4;
   const int32_t j0 = t / kRanked * per;
   const int32_t j1 = j0 + per < n ? j0 + per : n;
   if (e < n) {
     const uint64_t mine = s[e];
-    int32_t above = 0;
+    int32_t above = 0, before = 0;
 #pragma unroll 8
-    for (int32_t j = j0; j < j1; ++j) above += s[j] > mine ? 1 : 0;
+    for (int32_t j = j0; j < j1; ++j) {
+      const uint64_t other = s[j];
+      above += other > mine ? 1 : 0;
+      if (INDEXED) before += (uint32_t)other > (uint32_t)mine ? 1 : 0;
+    }
     if (above) atomicAdd(&rank[e], above);
+    if (INDEXED && before) atomicAdd(&by_index[e], before);
   }
   __syncthreads();
-  if (t < n) sorted[rank[t]] = s[t];  // (n <= kRanked; places differ)
+  if (t < n) {  // (n <= kRanked; places differ)
+    sorted[rank[t]] = s[t];
+    if (INDEXED) index_ranks(s)[rank[t]] = by_index[t];
+  }
   __syncthreads();
   return t < n ? sorted[t] : 0;
 }
@@ -958,7 +983,7 @@ __device__ __forceinline__ uint64_t cut_list(const Weights& w, const Params& q, 
   uint64_t x[P];
   const int t = threadIdx.x;
   if constexpr (P == 1) {
-    x[0] = rank_places(n, s.list.place);  // (at most kRanked)
+    x[0] = rank_places<true>(n, s.list.place);  // (at most kRanked)
   } else {
 #pragma unroll
     for (int e = 0; e < P; ++e) x[e] = t * P + e < n ? s.list.place[t * P + e] : 0;
@@ -1011,7 +1036,8 @@ __device__ __forceinline__ uint64_t cut_list(const Weights& w, const Params& q, 
     if (t * P + e == last) s.value64[2] = x[e];
   // (The sorted list stays in place for the caller.)
 #pragma unroll
-  for (int e = 0; e < P; ++e) s.list.place[t * P + e] = x[e];
+  for (int e = 0; e < P; ++e)
+    if (P > 1 || t < kRanked) s.list.place[t * P + e] = x[e];
   __syncthreads();
   return s.value64[2];
 }
@@ -1031,7 +1057,7 @@ __device__ __forceinline__ uint64_t members(int32_t n, int32_t bin, SubBin sub_b
     }
   __syncthreads();
   count = s.length;
-  return count <= kRanked ? rank_places(count, found) : 0;
+  return count <= kRanked ? rank_places<false>(count, found) : 0;
 }
 
 // The last kept place of a longer list: its tokens' counts and masses in sub-bins of equal key
@@ -1280,18 +1306,18 @@ __device__ __forceinline__ void finish_list(const SampleArgs& a, int64_t r, cons
                                             const Weights& w, uint64_t least, int32_t n,
                                             uint64_t last_place, RowShared& s) {
   const int t = threadIdx.x;
-  // By falling ~index, each with its key.
-  uint64_t* by_index = reinterpret_cast<uint64_t*>(&s.queue);
-  if (t < n) by_index[t] = (s.list.place[t] << 32) | (s.list.place[t] >> 32);
-  if (t == 0) {
-    s.value64[0] = 0;
-    s.value32[0] = 0;
+  uint64_t* place_at = reinterpret_cast<uint64_t*>(&s.queue);
+  uint64_t* mass_at = place_at + kRanked;
+  if (t < n) {
+    const uint64_t mine = s.list.place[t];
+    const uint64_t x = mine >= last_place ? w(value_of(place_key(mine))) : 0;
+    const int32_t at = index_ranks(s.list.place)[t];
+    place_at[at] = mine;
+    mass_at[at] = x >= least ? x : 0;
   }
   __syncthreads();
-  const uint64_t mine = rank_places(n, by_index);
-  const uint64_t place = (mine << 32) | (mine >> 32);
-  uint64_t mass = t < n && place >= last_place ? w(value_of(place_key(place))) : 0;
-  mass = mass >= least ? mass : 0;
+  const uint64_t place = t < n ? place_at[t] : 0;
+  const uint64_t mass = t < n ? mass_at[t] : 0;
   uint64_t total;
   const uint64_t before = workgroup_scan<kWaves, uint64_t>(mass, s.wave64, total);
   const uint64_t target = scaled(q.u, total);
@@ -1512,7 +1538,7 @@ __global__ __launch_bounds__(kThreads) void gather_kernel(SampleArgs a) {
   }
   const float from = bin_from(bin, top);
   if (t == 0) s.queue.length = 0;
-  if (tile_max >= from && tile_max > -INFINITY) s.visit[atomicAdd(&s.visits, 1)] = tile0 + t;
+  push_visit(tile_max >= from && tile_max > -INFINITY, tile0 + t, s.visit, &s.visits);
   __syncthreads();
   // The mass that a token adds to its tile, or its place in the list.
   const auto take = [&](float v, int32_t index) {
@@ -1656,7 +1682,7 @@ __global__ __launch_bounds__(kThreads) void row_kernel(SampleArgs a) {
         for (int32_t b = t; b < kBins; b += kThreads) s.list.bin_count[b] = 0;
       }
       const float from = bin_from(last, top);
-      if (tile_max >= from && tile_max > -INFINITY) s.visit[atomicAdd(&s.visits, 1)] = t;
+      push_visit(tile_max >= from && tile_max > -INFINITY, t, s.visit, &s.visits);
       __syncthreads();
       // (min-p alone lists nothing: its tokens' weights go to their tiles.)
       read_tiles_sparse(row, tiles, s.visit, s.visits, from, s.queue, [&](float v, int32_t index) {
