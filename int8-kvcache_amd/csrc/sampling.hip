@@ -320,11 +320,13 @@ __device__ __forceinline__ bool needs_list(const SampleArgs& a, const Params& q)
   return a.parts > 0 && !q.greedy && q.k > kLongList && q.k <= kList;
 }
 
-// Tokens waiting for their weights, so that those are computed by whole waves: value and index.
+// Tokens waiting for their weights, so that those are computed by whole waves: places in a round's
+// vectors, which lie beside them.
 constexpr int kQueue = 4096;
+constexpr int kTogether = 4;  // vectors per thread and round
 struct Queue {
-  float value[kQueue];
-  int32_t index[kQueue];
+  u32x4 raw[kTogether * kThreads];
+  uint16_t place[kQueue];
   int32_t length;
 };
 
@@ -510,8 +512,8 @@ __device__ __forceinline__ void read_tiles(const Row<DT>& row, const Tiles<DT>& 
                                            const int32_t* visit, int32_t visits, float from,
                                            Queue& queue, Token token, Whole whole) {
   constexpr int kE = Row<DT>::kE;
-  constexpr int kTogether = 4;
   constexpr uint32_t kDense = 64 * kTogether * kE / 2;
+  static_assert(kTogether * kThreads * kE <= 1 << 16, "a place has 16 bits");
   const int lane = threadIdx.x & 63;
   const int32_t items = visits << tiles.shift;
   const float least = fmaxf(from, -3.4028235e38f);
@@ -522,54 +524,65 @@ __device__ __forceinline__ void read_tiles(const Row<DT>& row, const Tiles<DT>& 
 #pragma unroll
   for (int u = 0; u < kTogether; ++u) raw[u] = row.request(slot_of(u * kThreads + (int32_t)threadIdx.x));
   for (int32_t i0 = 0; i0 < items; i0 += kTogether * kThreads) {
-    float v[kTogether][kE];
-    int32_t slot[kTogether];
     uint32_t hits = 0;  // one bit per value
 #pragma unroll
     for (int u = 0; u < kTogether; ++u) {
-      slot[u] = slot_of(i0 + u * kThreads + (int32_t)threadIdx.x);
-      if (slot[u] >= 0) {
-        row.template values<false>(slot[u], raw[u], v[u]);
+      const int32_t slot = slot_of(i0 + u * kThreads + (int32_t)threadIdx.x);
+      if (slot >= 0) {
+        float v[kE];
+        row.template values<false>(slot, raw[u], v);
 #pragma unroll
-        for (int j = 0; j < kE; ++j) hits |= v[u][j] >= least ? 1u << (u * kE + j) : 0u;
+        for (int j = 0; j < kE; ++j) hits |= v[j] >= least ? 1u << (u * kE + j) : 0u;
       }
+    }
+    uint32_t incl = wave_scan<uint32_t>((uint32_t)__popc(hits));
+    uint32_t all = last_lane(incl);
+    if (all > kDense) {  // (uniform)
+#pragma unroll
+      for (int u = 0; u < kTogether; ++u) {
+        const int32_t slot = slot_of(i0 + u * kThreads + (int32_t)threadIdx.x);
+        if (slot < 0) continue;
+        float v[kE];
+        row.template values<false>(slot, raw[u], v);
+        whole(v, (hits >> (u * kE)) & ((1u << kE) - 1), slot);
+      }
+      hits = 0;
+      all = 0;
+    } else if (all > 0) {
+#pragma unroll
+      for (int u = 0; u < kTogether; ++u) queue.raw[u * kThreads + threadIdx.x] = raw[u];
     }
 #pragma unroll
     for (int u = 0; u < kTogether; ++u)
       raw[u] = row.request(slot_of(i0 + (kTogether + u) * kThreads + (int32_t)threadIdx.x));
-    if (__builtin_amdgcn_readfirstlane(last_lane(wave_scan<uint32_t>((uint32_t)__popc(hits)))) > kDense) {
-#pragma unroll
-      for (int u = 0; u < kTogether; ++u)
-        if (slot[u] >= 0) whole(v[u], (hits >> (u * kE)) & ((1u << kE) - 1), slot[u]);
-      hits = 0;
-    }
     // (Barriers that leave the requests in flight.)
     for (int32_t found = kQueue + 1; found > kQueue;) {
-      const uint32_t n = (uint32_t)__popc(hits);
-      const uint32_t incl = wave_scan<uint32_t>(n);
-      const uint32_t all = last_lane(incl);
-      if (all > 0) {  // (uniform)
+      if (all > 0) {
         int32_t at = 0;
         if (lane == 63) at = atomicAdd(&queue.length, (int32_t)all);
-        at = (int32_t)last_lane((uint32_t)at) + (int32_t)(incl - n);
-#pragma unroll
-        for (int u = 0; u < kTogether; ++u)
-#pragma unroll
-          for (int j = 0; j < kE; ++j) {
-            constexpr uint32_t one = 1u;
-            if ((hits & (one << (u * kE + j))) && at < kQueue) {
-              queue.value[at] = v[u][j];
-              queue.index[at] = row.first(slot[u]) + j;
-              ++at;
-              hits &= ~(one << (u * kE + j));
-            }
-          }
+        at = (int32_t)last_lane((uint32_t)at) + (int32_t)(incl - (uint32_t)__popc(hits));
+        while (hits && at < kQueue) {
+          const int32_t b = __ffs((int)hits) - 1;
+          queue.place[at++] =
+              (uint16_t)((b / kE * kThreads + (int32_t)threadIdx.x) * kE + b % kE);
+          hits &= hits - 1;
+        }
       }
       lds_barrier();
       found = queue.length;
       if (found == 0) break;
       const int32_t queued = found < kQueue ? found : kQueue;
-      for (int32_t i = threadIdx.x; i < queued; i += kThreads) token(queue.value[i], queue.index[i]);
+      for (int32_t i = threadIdx.x; i < queued; i += kThreads) {
+        const int32_t place = queue.place[i];
+        const int32_t slot = slot_of(i0 + place / kE);
+        const int32_t index = row.first(slot) + place % kE;
+        const bool inner = slot >= 1 && slot <= row.vectors;
+        token(inner ? Row<DT>::value_in(queue.raw, place) : row.element(index), index);
+      }
+      if (found > kQueue) {  // what is left goes into the next turn
+        incl = wave_scan<uint32_t>((uint32_t)__popc(hits));
+        all = last_lane(incl);
+      }
       lds_barrier();
       if (threadIdx.x == 0) queue.length = 0;
       lds_barrier();
@@ -590,7 +603,6 @@ __device__ __forceinline__ void read_tiles_sparse(const Row<DT>& row, const Tile
                                                   const int32_t* visit, int32_t visits, float from,
                                                   SlotQueue& queue, Token token) {
   constexpr int kE = Row<DT>::kE;
-  constexpr int kTogether = 4;
   const int32_t items = visits << tiles.shift;
   const float least = fmaxf(from, -3.4028235e38f);
   const auto slot_of = [&](int32_t i) {
