@@ -190,13 +190,14 @@ struct Weights {
 // within the chunk both use it.
 struct FastWeights {
   double c, k;  // y = v c - k
-  float low;    // y = -100 here
+  float low;    // y is about -99.5 here: weight 0
   int32_t frac;
 
-  __device__ __forceinline__ FastWeights(float t, float top, int32_t fraction) {
-    c = 0x1.71547652b82fep+0 / (double)t;
+  // `rate`: log2(e) / t.
+  __device__ __forceinline__ FastWeights(double rate, float t, float top, int32_t fraction) {
+    c = rate;
     k = (double)top * c;
-    low = (float)((double)top - 100.0 / c);
+    low = top - 69.0f * t;  // (about 100 ln 2)
     frac = fraction;
   }
   // The maximum's weight is exactly 2^frac, and `low` lies below the maximum.
@@ -363,6 +364,7 @@ __global__ __launch_bounds__(kChunkThreads) void chunk_kernel(SampleArgs a) {
   if (run == 0 && threadIdx.x == 0) a.list_count[r] = 0;
   // Rows whose whole mass is needed: without a filter, and with a nucleus cut alone.
   const bool summed = !q.greedy && q.k == 0 && (q.p < 1.0 ? a.parts > 0 : !(q.m > 0.0));
+  const double rate = 0x1.71547652b82fep+0 / (double)q.t;
   for (int32_t c = c0; c < c1; ++c) {
     const int buf = c & 1;
     float v[kSteps][kE];
@@ -400,7 +402,7 @@ __global__ __launch_bounds__(kChunkThreads) void chunk_kernel(SampleArgs a) {
     if (summed) {
       uint64_t sum = 0;
       if (FastWeights::fits(q.t, top)) {
-        const FastWeights w(q.t, top, a.frac);
+        const FastWeights w(rate, q.t, top, a.frac);
         double part = 0x1p52;
 #pragma unroll
         for (int j = 0; j < kSteps; ++j)
@@ -408,7 +410,7 @@ __global__ __launch_bounds__(kChunkThreads) void chunk_kernel(SampleArgs a) {
           for (int e = 0; e < kE; ++e) part = w.add(v[j][e], part);
         sum = FastWeights::value(part);
       } else if (top > -INFINITY) {
-        const Weights w{0x1.71547652b82fep+0 / (double)q.t, (double)top, top, a.frac};
+        const Weights w{rate, (double)top, top, a.frac};
 #pragma unroll
         for (int j = 0; j < kSteps; ++j)
 #pragma unroll
@@ -1262,7 +1264,7 @@ __device__ __forceinline__ void finish_plain(const SampleArgs& a, const Row<DT>&
   uint64_t sum = 0;
   row.load(t < kChunkSlots ? slot : row.slots(), v);  // (past the row: -inf)
   if (FastWeights::fits(q.t, cm)) {
-    const FastWeights w(q.t, cm, a.frac);
+    const FastWeights w(c, q.t, cm, a.frac);
 #pragma unroll
     for (int j = 0; j < kE; ++j) x[j] = w(v[j]);
   } else {
