@@ -717,9 +717,9 @@ bool rows16(const void* p, int64_t stride) {
 
 // Parts of k.  Tiles of 16 tokens: about four workgroups of four waves per compute unit (32 tokens
 // on 24 adapters, the four projections of a layer: 35 us with 12-16 parts, 37 with 8, 56 with 2).
-// Tiles of 64: eight waves, as many workgroups as run at a time, two per unit up to rank 32 and one
-// above, where the registers leave room for no more (1100 tokens, 18944 x 3584, rank 32, 34 tiles:
-// 25.3 us with 14 parts, 27.8 with 7, 28.4 with 16; 1057 tokens, 18944 x 37888, rank 64, 20 tiles:
+// Tiles of 64: eight waves, as many workgroups as run at a time, nearly two per unit up to rank 32
+// and one above, where the registers leave room for no more (1100 tokens, 18944 x 3584, rank 32, 34
+// tiles: 24.3 us with 12 parts, 27.7 with 7, 27.9 with 16; 1057 tokens, 18944 x 37888, rank 64, 20 tiles:
 // 55 with 12, 62 with 16, 64 with 6).  A part has at least two steps per wave.
 int splits_for(int64_t tiles, int64_t k, int rows, int32_t rank) {
   const int64_t shortest = 2 * 32 * (rows == 16 ? kShrinkWaves<1> : kShrinkWaves<4>);
@@ -729,7 +729,7 @@ int splits_for(int64_t tiles, int64_t k, int rows, int32_t rank) {
     s = (1024 + tiles - 1) / (tiles > 0 ? tiles : 1);
     s = s < 16 ? s : 16;
   } else {
-    s = (rank <= 32 ? 480 : 256) / (tiles * ((rank + 63) / 64));
+    s = (rank <= 32 ? 416 : 256) / (tiles * ((rank + 63) / 64));
   }
   s = s < most ? s : most;
   return (int)(s < 1 ? 1 : s);
@@ -926,10 +926,13 @@ extern "C" int int8kv_lora_add(const void* base, int64_t base_row_stride, const 
   a.staged = nullptr;
   if (rows == 64) {
     launch_shrink<4>(a, s);
-    // The parts' sums in a launch of their own where the second product would read more than 32 MB
-    // of parts (1057 tokens, 18944 x 37888, rank 64, 776 MB: 105 us without, 64 with; 1100, 18944 x
-    // 3584, rank 32, 47 MB: 34.1 and 33.2; 523, 4096 x 4608, rank 32, 15 MB: 14.8 and 15.8).
-    if (tiles * a.groups * a.splits * rows * rank * 4 > 32 << 20) {
+    // The parts' sums in a launch of their own, where a workgroup of the second product would need
+    // more than four rounds of loads for them (148 tokens, 18944 x 3584, rank 64, 32 parts: 31.6 us
+    // without, 19.4 with; 3294, 3936 x 4608, rank 128, 2 parts: 61.6 and 50.9; 500, 4096 x 4096,
+    // rank 32, 8 parts, two rounds: 13.7 and 15.0), or all of them would read more than 32 MB of
+    // parts (4907, 2048 x 3584, rank 32: 34.5 and 31.8; 6007, 3584 x 37888, rank 64: 232 and 226).
+    const int64_t rounds = rank / 16 * ((a.splits + 7) / 8);
+    if (rounds > 4 || tiles * a.groups * a.splits * rows * rank * 4 > 32 << 20) {
       a.staged = reinterpret_cast<uint16_t*>(a.part + (int64_t)a.splits * tiles * rows * rank);
       const int64_t quads = tiles * rows * rank / 4;
       hipLaunchKernelGGL(sum_kernel, dim3((unsigned)((quads + kSumThreads - 1) / kSumThreads)),
