@@ -53,9 +53,9 @@ struct Plan {
 };
 
 // Tokens per tile: 16 (one matrix tile), or 64 where the adapters have 32 tokens or more each: an
-// adapter's weights are then read for 64 tokens at a time (6007 tokens on 5 adapters, rank 64,
-// 3584 x 37888: 595 us with tiles of 16, most of it the traffic of B, 454 with 64 and nothing else
-// changed); below that the tiles would be mostly empty.
+// adapter's weights are then read for 64 tokens at a time where that counts (6007 tokens on 5
+// adapters, rank 64, 3584 x 37888: 595 us with tiles of 16, most of it the traffic of B, 454 with 64
+// and nothing else changed); below that the tiles would be mostly empty.
 int tile_rows(int64_t tokens, int32_t adapters) {
   return tokens >= 32 * (int64_t)adapters && tokens >= 64 ? 64 : 16;
 }
@@ -191,6 +191,8 @@ struct LoraArgs {
   float* part;  // [splits][tiles x rows of a tile][rank]
   uint16_t* staged;  // [tiles x rows of a tile][2][rank]: their sums in two parts, or null
   Plan plan;
+  int32_t tiles;       // of the products: the plan's, or its quarters (tile_shift 2)
+  int32_t tile_shift;
   int32_t k, n, rank;
   int32_t splits;  // parts of k
   int32_t chunk;   // k of a part (a multiple of 32)
@@ -215,6 +217,16 @@ __device__ __forceinline__ void store16(uint16_t* p, u32x4 v) {
   else
     *reinterpret_cast<u32x4*>(p) = v;
 }
+// {adapter, rows} of a tile of 16 x TT tokens.
+template <int TT>
+__device__ __forceinline__ int2 head_of(const LoraArgs& a, int32_t tile) {
+  int2 head = a.plan.head[TT == 1 ? tile >> a.tile_shift : tile];
+  if constexpr (TT == 1) {
+    const int32_t rows = head.y - 16 * (tile & ((1 << a.tile_shift) - 1));
+    head.y = rows < 0 ? 0 : (rows < 16 ? rows : 16);
+  }
+  return head;
+}
 __device__ __forceinline__ bf16x8 zero8() {
   return __builtin_bit_cast(bf16x8, u32x4{0u, 0u, 0u, 0u});
 }
@@ -238,13 +250,13 @@ __global__ __launch_bounds__(kShrinkWaves<TT> * 64) void shrink_kernel(LoraArgs 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i = lane & 15;
   const int g = lane >> 4;
-  const int2 head = a.plan.head[tile];
+  const int2 head = head_of<TT>(a, tile);
   int32_t token[TT];
 #pragma unroll
   for (int tt = 0; tt < TT; ++tt) token[tt] = a.plan.token[tile * kRows + 16 * tt + i];
   const int32_t adapter = __builtin_amdgcn_readfirstlane(head.x);
   const int32_t rows = __builtin_amdgcn_readfirstlane(head.y);
-  if (adapter < 0) return;  // (unused tiles too)
+  if (adapter < 0 || rows == 0) return;
   const int32_t first = __builtin_amdgcn_readlane(token[0], 0);
   const uint16_t* xp[TT];
 #pragma unroll
@@ -316,7 +328,7 @@ __global__ __launch_bounds__(kShrinkWaves<TT> * 64) void shrink_kernel(LoraArgs 
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
         const int32_t r = r0 + 16 * rt + 4 * g;
-        const int64_t row = ((int64_t)split * a.plan.tiles + tile) * kRows + 16 * tt + i;
+        const int64_t row = ((int64_t)split * a.tiles + tile) * kRows + 16 * tt + i;
         if (16 * tt + i < rows && r < a.rank)
           *reinterpret_cast<f32x4*>(a.part + row * a.rank + r) = acc[tt][rt];
       }
@@ -351,7 +363,7 @@ __global__ __launch_bounds__(kSumThreads) void sum_kernel(LoraArgs a, int32_t ro
   constexpr int kTogether = 8;
   const int32_t quads = a.rank / 4;
   const int64_t q = (int64_t)blockIdx.x * kSumThreads + threadIdx.x;
-  const int64_t all = (int64_t)a.plan.tiles * rows * quads;
+  const int64_t all = (int64_t)a.tiles * rows * quads;
   if (q >= all) return;
   const f32x4* part = reinterpret_cast<const f32x4*>(a.part);
   f32x4 h = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -400,8 +412,8 @@ __global__ __launch_bounds__(kExpandWaves * 64) void expand_kernel(LoraArgs a) {
     group = blockIdx.x - tile * a.groups;
   } else {
     const int32_t at = blockIdx.x / kXcds;
-    const int32_t round = at / a.plan.tiles;
-    tile = at - round * a.plan.tiles;
+    const int32_t round = at / a.tiles;
+    tile = at - round * a.tiles;
     group = round * kXcds + blockIdx.x % kXcds;
     if (group >= a.groups) return;
   }
@@ -411,7 +423,7 @@ __global__ __launch_bounds__(kExpandWaves * 64) void expand_kernel(LoraArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i = lane & 15;
   const int g = lane >> 4;
-  const int2 head = a.plan.head[tile];
+  const int2 head = head_of<TT>(a, tile);
   // As an operand lane (i, g) holds token i; in base and out lane l holds columns 8 (l % 8) .. + 7
   // of rows l / 8 and 8 + l / 8.
   const int line = lane >> 3;
@@ -423,7 +435,7 @@ __global__ __launch_bounds__(kExpandWaves * 64) void expand_kernel(LoraArgs a) {
   // The tile's vectors, four values per thread and round (those behind its rows are not set; they
   // meet no other row).
   const int32_t quads = a.rank / 4;
-  const int64_t split_stride = (int64_t)a.plan.tiles * kRows * a.rank;
+  const int64_t split_stride = (int64_t)a.tiles * kRows * a.rank;
   const float* part = a.part + (int64_t)tile * kRows * a.rank;
   constexpr int kTogether = 8;  // partial sums requested together
   f32x4 y[kTogether];
@@ -602,7 +614,7 @@ __global__ __launch_bounds__(kBothWaves * 64) void both_kernel(LoraArgs a) {
   const int i = lane & 15;
   const int g = lane >> 4;
   const int line = lane >> 3;
-  const int2 head = a.plan.head[tile];
+  const int2 head = head_of<1>(a, tile);
   const int32_t mine = a.plan.token[tile * 16 + i];
   int32_t token[2];
 #pragma unroll
@@ -735,6 +747,16 @@ int splits_for(int64_t tiles, int64_t k, int rows, int32_t rank) {
   return (int)(s < 1 ? 1 : s);
 }
 
+// A plan's tiles of 64 tokens as four of 16, which have more workgroups with shorter chains but
+// read A and B four times as often: up to 96 MB of that (16000 tokens, 512 x 512, rank 8, 17 MB: 12.4
+// us, 26.2 in tiles of 64; 512, 3584 x 4608, rank 16, 13 MB: 9.7 and 12.1; 4942, 512 x 4376, rank
+// 24, 74 MB: 30.4 and 35.2; 2000, 3584 x 4608, rank 32, 75 MB: 23.9 and 23.4; 160, 3584 x 37888,
+// rank 64, 106 MB: 22.5 and 22.7; 1100, 18944 x 3584, rank 32, 196 MB: 36.9 and 33.3; 3000, 4096 x
+// 4096, rank 64, 231 MB: 41.1 and 31.8).
+bool taken_as_quarters(int64_t tiles, int64_t k, int32_t rank, int64_t n) {
+  return 4 * tiles * rank * (k + n) * 2 <= 96 << 20;
+}
+
 // Both products in one launch?  A launch costs about 2.5 us and one compute unit loads A at about
 // 30 bytes a ns, so where an adapter's A has at most 64 KB, and all workgroups' together 64 KB per
 // compute unit (one token: 1024 x 4096, rank 8: 6.6 us in two launches, 4.2 in one; 2048 x 4608,
@@ -754,7 +776,7 @@ bool lora_sizes_ok(int64_t tokens, int32_t adapters, int64_t k, int32_t rank) {
 
 template <int TT>
 void launch_shrink(const LoraArgs& a, hipStream_t s) {
-  const dim3 grid((unsigned)((int64_t)a.plan.tiles * a.splits * a.halves)), block(kShrinkWaves<TT> * 64);
+  const dim3 grid((unsigned)((int64_t)a.tiles * a.splits * a.halves)), block(kShrinkWaves<TT> * 64);
   if (a.rank <= 16)
     hipLaunchKernelGGL((shrink_kernel<TT, 1>), grid, block, 0, s, a);
   else if (a.rank <= 32)
@@ -764,7 +786,7 @@ void launch_shrink(const LoraArgs& a, hipStream_t s) {
 }
 
 void launch_both(const LoraArgs& a, hipStream_t s) {
-  const dim3 grid((unsigned)(a.plan.tiles * a.groups)), block(kBothWaves * 64);
+  const dim3 grid((unsigned)((int64_t)a.tiles * a.groups)), block(kBothWaves * 64);
   const bool paired = a.rank % 32 == 0;
   switch ((2 * a.rank + 31) / 32) {
 #define INT8KV_BOTH(RT, NS, PAIRED) \
@@ -784,7 +806,7 @@ void launch_both(const LoraArgs& a, hipStream_t s) {
 template <int TT, bool STREAM>
 void launch_expand(const LoraArgs& a, hipStream_t s) {
   const int64_t groups = TT == 1 ? a.groups : (a.groups + kXcds - 1) / kXcds * kXcds;
-  const dim3 grid((unsigned)(a.plan.tiles * groups)), block(kExpandWaves * 64);
+  const dim3 grid((unsigned)(a.tiles * groups)), block(kExpandWaves * 64);
   const bool paired = a.rank % 32 == 0;
   switch ((2 * a.rank + 31) / 32) {
 #define INT8KV_EXPAND(NS, PAIRED) \
@@ -856,7 +878,12 @@ extern "C" size_t int8kv_lora_workspace_bytes(int64_t tokens, int32_t num_adapte
   if (!lora_sizes_ok(tokens, num_adapters, k, rank)) return 0;
   const int rows = tile_rows(tokens, num_adapters);
   const int64_t tiles = max_tiles(tokens, num_adapters, rows);
-  return 16 + (size_t)tiles * rows * rank * 4 * (splits_for(tiles, k, rows, rank) + (rows == 64 ? 1 : 0));
+  int64_t parts = splits_for(tiles, k, rows, rank);
+  if (rows == 64) {  // with their sums, or taken as quarters
+    const int64_t quarters = splits_for(4 * tiles, k, 16, rank);
+    parts = parts + 1 > quarters ? parts + 1 : quarters;
+  }
+  return 16 + (size_t)(tiles * rows * rank * 4 * parts);
 }
 
 extern "C" int int8kv_lora_add(const void* base, int64_t base_row_stride, const void* x,
@@ -905,8 +932,16 @@ extern "C" int int8kv_lora_add(const void* base, int64_t base_row_stride, const 
   a.k = (int32_t)k;
   a.n = (int32_t)n;
   a.rank = rank;
-  const int64_t tiles = a.plan.tiles;
-  const int rows = tile_rows(tokens, num_adapters);
+  int64_t tiles = a.plan.tiles;
+  int rows = tile_rows(tokens, num_adapters);
+  a.chunks = (int32_t)((n + kExpandColumns - 1) / kExpandColumns);
+  a.tile_shift = 0;
+  if (rows == 64 && taken_as_quarters(tiles, k, rank, n)) {
+    rows = 16;
+    a.tile_shift = 2;
+    tiles *= 4;
+  }
+  a.tiles = (int32_t)tiles;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (both_at_once(tiles, rows, k, rank, n)) {
     a.groups = (int32_t)((n + kBothColumns - 1) / kBothColumns);
@@ -916,7 +951,6 @@ extern "C" int int8kv_lora_add(const void* base, int64_t base_row_stride, const 
   a.splits = splits_for(tiles, k, rows, rank);
   a.chunk = (int32_t)(((k + a.splits - 1) / a.splits + 31) / 32 * 32);
   a.halves = (rank + 63) / 64;
-  a.chunks = (int32_t)((n + kExpandColumns - 1) / kExpandColumns);
   // Runs of chunks: while there are about fourteen workgroups per compute unit (99 tiles of 148
   // chunks: runs of 4 240 us, 2 255, 8 265, 1 300).
   int64_t run = rows == 16 ? 1 : tiles * a.chunks / 3584;

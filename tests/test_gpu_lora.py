@@ -232,3 +232,21 @@ def test_more_tokens_than_a_plan_holds(cuda, tokens, adapters, run):
     ids = torch.randint(-1, adapters, (tokens // run + 1,), generator=g).repeat_interleave(run)[:tokens]
     d = inputs(cuda, tokens, 40, 24, 8, adapters, seed=13, ids=ids)
     check(d, add(d))
+
+
+@pytest.mark.parametrize("tokens,k,n,rank,adapters", [
+    (200, 264, 136, 24, 3),       # tiles of 64 taken as quarters, one launch
+    (130, 4104, 264, 32, 2),      # as quarters, two launches
+    (96, 1032, 264, 128, 1),
+    (3000, 2048, 264, 128, 5),    # whole tiles (122 MB as quarters), the parts summed beforehand
+    (2500, 3000, 520, 56, 40),    # whole tiles, no sums
+])
+def test_whole_tiles_and_quarters(cuda, tokens, k, n, rank, adapters):
+    """Tiles of 64 tokens in both readings, with partly filled ones, out in place and not."""
+    d = inputs(cuda, tokens, k, n, rank, adapters, seed=tokens)
+    want = add(d)
+    check(d, want)
+    none = (d["ids"] < 0) | (d["ids"] >= adapters)
+    d["x"][none] = float("nan")
+    out = add(d, out=d["base"])
+    assert out.data_ptr() == d["base"].data_ptr() and torch.equal(out, want)
