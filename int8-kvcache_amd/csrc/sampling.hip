@@ -901,53 +901,6 @@ struct RowShared {
   int32_t visits, length;
 };
 
-// Sorts N = kThreads * P places, largest first: value e of thread t is number t P + e.  Partners
-// within a thread by registers, within a wave by lane exchange, else through LDS.
-template <int P>
-__device__ __forceinline__ void sort_places(uint64_t (&x)[P], uint64_t* s) {
-  constexpr int kN = kThreads * P;
-  const int t = threadIdx.x;
-  for (int size = 2; size <= kN; size <<= 1) {
-    for (int step = size >> 1; step >= 1; step >>= 1) {
-      if (step >= 64 * P) {
-        __syncthreads();
-#pragma unroll
-        for (int e = 0; e < P; ++e) s[t * P + e] = x[e];
-        __syncthreads();
-      }
-      if (step >= P) {
-#pragma unroll
-        for (int e = 0; e < P; ++e) {
-          const int i = t * P + e;
-          const uint64_t y = step >= 64 * P
-                                 ? s[i ^ step]
-                                 : (uint64_t)__shfl_xor((unsigned long long)x[e], step / P, 64);
-          const bool larger = ((i & size) == 0) == ((i & step) == 0);
-          x[e] = (y > x[e]) == larger ? y : x[e];
-        }
-      } else if constexpr (P > 1) {
-#pragma unroll
-        for (int e = 0; e < P; ++e) {
-          const int i = t * P + e;
-          const int o = e ^ step;
-          if (o > e) {  // (step is 1 or 2: resolved when unrolled over both)
-            const bool down = (i & size) == 0;
-            uint64_t lo = x[0], hi = x[0];
-#pragma unroll
-            for (int z = 0; z < P; ++z) {
-              lo = z == e ? x[z] : lo;
-              hi = z == o ? x[z] : hi;
-            }
-            const bool swap = (hi > lo) == down && hi != lo;
-#pragma unroll
-            for (int z = 0; z < P; ++z) x[z] = swap ? (z == e ? hi : (z == o ? lo : x[z])) : x[z];
-          }
-        }
-      }
-    }
-  }
-}
-
 // The order of at most kRanked places: four threads per place count the larger ones.  INDEXED: the
 // places' numbers by index too, left behind (index_ranks) in the order of the places.
 constexpr int kRanked = kThreads / 4;
@@ -994,68 +947,38 @@ struct ListCut {
   uint64_t all_mass;
 };
 
-// Sorts the list's n places and finds the last kept one.
-template <int P>
-__device__ __forceinline__ uint64_t cut_list(const Weights& w, const Params& q, const ListCut& cut, int32_t n,
-                             RowShared& s) {
-  uint64_t x[P];
+// Sorts the list's n places (at most kRanked) and finds the last kept one.
+__device__ __forceinline__ uint64_t cut_short_list(const Weights& w, const Params& q,
+                                                   const ListCut& cut, int32_t n, RowShared& s) {
   const int t = threadIdx.x;
-  if constexpr (P == 1) {
-    x[0] = rank_places<true>(n, s.list.place);  // (at most kRanked)
-  } else {
-#pragma unroll
-    for (int e = 0; e < P; ++e) x[e] = t * P + e < n ? s.list.place[t * P + e] : 0;
-    sort_places<P>(x, s.list.place);
-  }
-  uint64_t weight[P];
-  uint64_t sum = 0;
-#pragma unroll
-  for (int e = 0; e < P; ++e) {
-    weight[e] = t * P + e < n ? w(value_of(place_key(x[e]))) : 0;
-    sum += weight[e];
-  }
+  const uint64_t x = rank_places<true>(n, s.list.place);
+  const uint64_t weight = t < n ? w(value_of(place_key(x))) : 0;
   __syncthreads();
   uint64_t total;
-  const uint64_t before = workgroup_scan<kWaves, uint64_t>(sum, s.wave64, total);
+  const uint64_t before = workgroup_scan<kWaves, uint64_t>(weight, s.wave64, total);
   // S(n_k): of the first k, or everything.
-  const bool top_k = q.k > 0 && q.k < n;
-  int32_t last = top_k ? q.k - 1 : n - 1;
+  int32_t last = q.k > 0 && q.k < n ? q.k - 1 : n - 1;
   if (t == 0) {
     s.value32[0] = -1;
     s.value64[2] = 0;
   }
   __syncthreads();
   if (q.p < 1.0) {
-    uint64_t at = before;
-#pragma unroll
-    for (int e = 0; e < P; ++e) {
-      at += weight[e];
-      if (t * P + e == last) s.value64[0] = at;
-    }
+    if (t == last) s.value64[0] = before + weight;
     __syncthreads();
     const uint64_t kept = q.k > 0 || cut.all_mass == 0 ? s.value64[0] : cut.all_mass;
     // Tokens whose preceding mass is below p S(n_k).
     uint64_t want = (uint64_t)ceil(q.p * (double)kept);
     want = want < 1 ? 1 : want;
-    at = cut.before + before;
-#pragma unroll
-    for (int e = 0; e < P; ++e) {
-      const bool first = at < want;
-      at += weight[e];
-      // (One of them: the token that reaches `want`, or the list's last.)
-      if (first && (at >= want || t * P + e == n - 1) && t * P + e < n) s.value32[0] = t * P + e;
-    }
+    const uint64_t at = cut.before + before;
+    // (One of them: the token that reaches `want`, or the list's last.)
+    if (at < want && (at + weight >= want || t == n - 1) && t < n) s.value32[0] = t;
     __syncthreads();
     last = s.value32[0] < last ? s.value32[0] : last;
   }
   __syncthreads();
-#pragma unroll
-  for (int e = 0; e < P; ++e)
-    if (t * P + e == last) s.value64[2] = x[e];
-  // (The sorted list stays in place for the caller.)
-#pragma unroll
-  for (int e = 0; e < P; ++e)
-    if (P > 1 || t < kRanked) s.list.place[t * P + e] = x[e];
+  if (t == last) s.value64[2] = x;
+  if (t < kRanked) s.list.place[t] = x;  // (the sorted list stays in place for the caller)
   __syncthreads();
   return s.value64[2];
 }
@@ -1078,13 +1001,115 @@ __device__ __forceinline__ uint64_t members(int32_t n, int32_t bin, SubBin sub_b
   return count <= kRanked ? rank_places<false>(count, found) : 0;
 }
 
+// The place, among those of the list within [low, high], at which their number (BY_MASS: their mass)
+// reaches `want`; `upto` is their mass up to it.  2048 sub-bins of equal ranges of places between
+// the outermost ones, again within the one that is reached, until that can be put in order: equal
+// logits differ in their indices, so two turns are the rule.
+constexpr int kSub = 2 * kThreads;
+static_assert(kSub <= kBins, "the row's bins are reused");
+template <bool BY_MASS>
+__device__ __forceinline__ uint64_t narrow(const Weights& w, bool weighed, int32_t n, uint64_t low,
+                                           uint64_t high, uint64_t want, RowShared& s,
+                                           uint64_t& upto) {
+  const int t = threadIdx.x;
+  uint64_t mass_before = 0;
+  for (;;) {
+    const auto within = [&](uint64_t place) { return place >= low && place <= high; };
+    uint64_t first = 0, last = ~0ull;
+    for (int32_t i = t; i < n; i += kThreads) {
+      const uint64_t p = s.list.place[i];
+      if (within(p)) {
+        first = p > first ? p : first;
+        last = p < last ? p : last;
+      }
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint64_t f = __shfl_xor((unsigned long long)first, d, 64);
+      const uint64_t l = __shfl_xor((unsigned long long)last, d, 64);
+      first = f > first ? f : first;
+      last = l < last ? l : last;
+    }
+    __syncthreads();
+    if (t == 0) {
+      s.value64[2] = 0;
+      s.value64[3] = ~0ull;
+    }
+    for (int32_t b = t; b < kSub; b += kThreads) {
+      s.list.bin_mass[b] = 0;
+      s.list.bin_count[b] = 0;
+    }
+    __syncthreads();
+    if ((t & 63) == 0) {
+      atomicMax(reinterpret_cast<unsigned long long*>(&s.value64[2]), (unsigned long long)first);
+      atomicMin(reinterpret_cast<unsigned long long*>(&s.value64[3]), (unsigned long long)last);
+    }
+    __syncthreads();
+    high = s.value64[2];
+    low = s.value64[3];
+    const uint64_t range = high - low;
+    const int shift = range < (uint64_t)kSub ? 0 : 64 - 11 - __clzll((long long)range);
+    const auto sub_bin = [&](uint64_t place) {
+      return within(place) ? (int32_t)((high - place) >> shift) : -1;
+    };
+    for (int32_t i = t; i < n; i += kThreads) {
+      const uint64_t p = s.list.place[i];
+      const int32_t b = sub_bin(p);
+      if (b < 0) continue;
+      atomicAdd(&s.list.bin_count[b], 1u);
+      if (weighed)
+        atomicAdd(reinterpret_cast<unsigned long long*>(&s.list.bin_mass[b]),
+                  (unsigned long long)w(value_of(place_key(p))));
+    }
+    __syncthreads();
+    const uint32_t c0 = s.list.bin_count[2 * t], c1 = s.list.bin_count[2 * t + 1];
+    const uint64_t m0 = s.list.bin_mass[2 * t], m1 = s.list.bin_mass[2 * t + 1];
+    uint32_t count_all;
+    uint64_t mass_all;
+    const uint32_t cb = workgroup_scan<kWaves, uint32_t>(c0 + c1, s.wave32, count_all);
+    const uint64_t mb = workgroup_scan<kWaves, uint64_t>(m0 + m1, s.wave64, mass_all);
+    const uint64_t x0 = BY_MASS ? mb : (uint64_t)cb;
+    const uint64_t x1 = x0 + (BY_MASS ? m0 : (uint64_t)c0);
+    const uint64_t x2 = x1 + (BY_MASS ? m1 : (uint64_t)c1);
+    if (x0 < want && want <= x2) {  // one thread
+      const bool second = x1 < want;
+      s.value32[6] = second ? 2 * t + 1 : 2 * t;
+      s.value64[0] = second ? mb + m0 : mb;
+      s.value64[1] = want - (second ? x1 : x0);
+    }
+    __syncthreads();
+    const int32_t bin = s.value32[6];
+    mass_before += s.value64[0];
+    want = s.value64[1];
+    int32_t count;
+    const uint64_t place = members(n, bin, sub_bin, s, count);
+    if (count > kRanked) {
+      low = high - ((uint64_t)bin << shift) - ((1ull << shift) - 1);  // (may wrap below 0: clamped)
+      if (low > high) low = 0;
+      high -= (uint64_t)bin << shift;
+      __syncthreads();
+      continue;
+    }
+    const uint64_t mass = weighed && t < count ? w(value_of(place_key(place))) : 0;
+    uint64_t sum;
+    const uint64_t at = workgroup_scan<kWaves, uint64_t>(mass, s.wave64, sum);
+    if (BY_MASS ? at < want && want <= at + mass : t + 1 == (int32_t)want) {  // one thread
+      s.value64[0] = place;
+      s.value64[1] = mass_before + at + mass;
+    }
+    __syncthreads();
+    upto = s.value64[1];
+    const uint64_t found = s.value64[0];
+    __syncthreads();
+    return found;
+  }
+}
+
 // The last kept place of a longer list: its tokens' counts and masses in sub-bins of equal key
-// ranges, then the exact order within the two sub-bins where the cuts fall.  False if one of those
-// holds too many (equal logits).
-__device__ __forceinline__ bool cut_by_bins(const Weights& w, const Params& q, const ListCut& cut,
-                                            int32_t n, RowShared& s, uint64_t& last) {
-  constexpr int kSub = 2 * kThreads;
-  static_assert(kSub <= kBins, "the row's bins are reused");
+// ranges, then the exact order within the two sub-bins where the cuts fall.
+__device__ __forceinline__ uint64_t cut_by_bins(const Weights& w, const Params& q,
+                                                const ListCut& cut, int32_t n, RowShared& s) {
+  uint64_t last;
   const int t = threadIdx.x;
   uint32_t high = 0, low = 0xffffffffu;
   for (int32_t i = t; i < n; i += kThreads) {
@@ -1112,6 +1137,14 @@ __device__ __forceinline__ bool cut_by_bins(const Weights& w, const Params& q, c
   const uint32_t range = high - s.wave32[1];
   const int shift = range < (uint32_t)kSub ? 0 : 32 - 11 - __clz((int)range);  // range >> shift < kSub
   const auto sub_bin = [&](uint64_t place) { return (int32_t)((high - place_key(place)) >> shift); };
+  // The places that a sub-bin can hold.
+  const auto highest = [&](int32_t bin) {
+    return ((uint64_t)(high - ((uint32_t)bin << shift)) << 32) | 0xffffffffu;
+  };
+  const auto lowest = [&](int32_t bin) {
+    const uint32_t key = high - ((uint32_t)bin << shift), width = (1u << shift) - 1;
+    return (uint64_t)(key > width ? key - width : 0) << 32;
+  };
   for (int32_t i = t; i < n; i += kThreads) {
     const uint64_t p = s.list.place[i];
     const int32_t b = sub_bin(p);
@@ -1142,17 +1175,23 @@ __device__ __forceinline__ bool cut_by_bins(const Weights& w, const Params& q, c
     __syncthreads();
     const int32_t left = s.value32[7];
     kept = s.value64[0];
-    const uint64_t place = members(n, s.value32[6], sub_bin, s, count);
-    if (count > kRanked) return false;
-    if (t == left - 1) s.value64[1] = place;
-    uint64_t sum = 0;
-    if (q.p < 1.0)
-      workgroup_scan<kWaves, uint64_t>(t < left ? w(value_of(place_key(place))) : 0, s.wave64, sum);
-    else
+    const int32_t bin = s.value32[6];
+    const uint64_t place = members(n, bin, sub_bin, s, count);
+    if (count > kRanked) {
+      uint64_t upto;
+      last = narrow<false>(w, q.p < 1.0, n, lowest(bin), highest(bin), (uint64_t)left, s, upto);
+      kept += upto;
+    } else {
+      if (t == left - 1) s.value64[1] = place;
+      uint64_t sum = 0;
+      if (q.p < 1.0)
+        workgroup_scan<kWaves, uint64_t>(t < left ? w(value_of(place_key(place))) : 0, s.wave64, sum);
+      else
+        __syncthreads();
+      kept += sum;
+      last = s.value64[1];
       __syncthreads();
-    kept += sum;
-    last = s.value64[1];
-    __syncthreads();
+    }
   } else if (q.k == 0 && cut.all_mass > 0) {
     kept = cut.all_mass;
   }
@@ -1168,8 +1207,12 @@ __device__ __forceinline__ bool cut_by_bins(const Weights& w, const Params& q, c
     }
     __syncthreads();
     const uint64_t before_bin = s.value64[0];
-    const uint64_t place = members(n, s.value32[6], sub_bin, s, count);
-    if (count > kRanked) return false;
+    const int32_t bin = s.value32[6];
+    const uint64_t place = members(n, bin, sub_bin, s, count);
+    if (count > kRanked) {
+      uint64_t upto;
+      return narrow<true>(w, true, n, lowest(bin), highest(bin), want - before_bin, s, upto);
+    }
     const uint64_t mass = t < count ? w(value_of(place_key(place))) : 0;
     uint64_t sum;
     const uint64_t at = before_bin + workgroup_scan<kWaves, uint64_t>(mass, s.wave64, sum);
@@ -1178,15 +1221,12 @@ __device__ __forceinline__ bool cut_by_bins(const Weights& w, const Params& q, c
     last = s.value64[1];
     __syncthreads();
   }
-  return true;
+  return last;
 }
 
-__device__ __forceinline__ uint64_t cut_list_any(const Weights& w, const Params& q,
-                                                 const ListCut& cut, int32_t n, RowShared& s) {
-  if (n <= kRanked) return cut_list<1>(w, q, cut, n, s);
-  uint64_t last;
-  if (cut_by_bins(w, q, cut, n, s, last)) return last;
-  return cut_list<kList / kThreads>(w, q, cut, n, s);
+__device__ __forceinline__ uint64_t cut_list(const Weights& w, const Params& q, const ListCut& cut,
+                                             int32_t n, RowShared& s) {
+  return n <= kRanked ? cut_short_list(w, q, cut, n, s) : cut_by_bins(w, q, cut, n, s);
 }
 
 // The first token, in index order, at which the kept weight exceeds `target`, within the slots
@@ -1749,7 +1789,7 @@ __global__ __launch_bounds__(kThreads) void row_kernel(SampleArgs a) {
       finish_general<DT>(copy, r, top, s);
       return;
     }
-    last_place = cut_list_any(w, q, cut, n, s);
+    last_place = cut_list(w, q, cut, n, s);
     if (!counted && n <= kRanked) {
       finish_list(a, r, q, w, least, n, last_place, s);
       return;
@@ -1838,14 +1878,16 @@ void plan_launches(SampleArgs& a) {
   a.run_chunks = (int32_t)(per_unit < 1 ? 1 : (per_unit < 8 ? per_unit : 8));
   a.runs = (a.chunks + a.run_chunks - 1) / a.run_chunks;
   // The histogram pass and the gathering behind it run where some row may have a nucleus cut alone
-  // and more tokens than its list holds.  A compute unit takes one of their workgroups; parts for
-  // twice the units, since rows with other settings leave at once (61 rows of mixed settings: 13 us
-  // each with 8 parts, 18 with 4), unless two rows out of three would wait for a second turn (200
-  // rows, all with a nucleus cut: 23 and 19 us with 1 part, 25 and 23 with 2).
+  // and more tokens than its list holds.  A compute unit takes one of their workgroups.  Without a
+  // top-k in the call every row may be such a one: one turn of the units (120 rows of 50257: 13 and
+  // 11 us with 2 parts, 16 and 18 with 4, 18 and 15 with 1).  With one, rows of other settings leave
+  // at once: up to two turns (61 rows of mixed settings, 152064: 11 and 13 us with 8 parts, 16 and 16
+  // with 4, 9 and 16 with 12).
   a.parts = 0;
   if (a.top_p && a.pieces > kList / kPieceElements) {
     const int64_t most = (a.vocab + 4 * kThreads - 1) / (4 * kThreads);
-    const int64_t want = a.rows <= 128 ? 512 / a.rows : (256 / a.rows < 1 ? 1 : 256 / a.rows);
+    const int64_t turns = a.top_k && a.rows <= 128 ? 512 : 256;
+    const int64_t want = turns / a.rows < 1 ? 1 : turns / a.rows;
     a.parts = (int32_t)(want < most ? want : most);
   }
 }

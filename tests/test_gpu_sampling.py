@@ -118,6 +118,19 @@ def test_many_ties_at_the_cut(cuda):
             both(cuda, logits, u, **kw)
 
 
+def test_hundreds_of_equal_logits(cuda):
+    """Lists whose cut falls among hundreds to thousands of equal logits, put in order by index."""
+    g = torch.Generator().manual_seed(17)
+    for dtype in DTYPES:
+        for vocab, steps in ((9000, 4.0), (30000, 16.0), (152064, 32.0), (152064, 64.0)):
+            logits = torch.round(torch.randn(12, vocab, generator=g) * 2.0 * steps) / steps
+            u = torch.rand(12, generator=g)
+            for kw in ({"top_k": 700}, {"top_k": 3500}, {"top_p": 0.5}, {"top_p": 0.93},
+                       {"top_k": 2900, "top_p": 0.8}, {"top_k": 1200, "top_p": 0.999, "min_p": 0.01},
+                       {"top_k": 4000, "top_p": 0.4, "temperature": 3.0}):
+                both(cuda, logits.to(dtype), u, **kw)
+
+
 def test_dense_values_at_the_cut(cuda):
     """Many distinct values close together (fp32), far from zero and around it."""
     g = torch.Generator().manual_seed(4)
