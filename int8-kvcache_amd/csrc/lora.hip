@@ -12,10 +12,10 @@
 // rounding to bf16 does.
 //
 // Bound: for few tokens by the adapters' bytes and two launches (one token, 3584 x 4608, rank 16:
-// 7.5 us, where a launch that exits at once takes 2 to 3; 1100 tokens on 16 adapters, 18944 x 3584,
-// rank 32: 25.3 us, whose bytes alone take 14.4 at a copy's rate); for many by reading the base and
-// writing the result (6007 tokens, 3584 x 37888: 229 us, of them 214 in the second product at
-// 4.3 TB/s).
+// 7.4 us, where a launch that exits at once takes 2 to 3; 1100 tokens on 16 adapters, 18944 x 3584,
+// rank 32: 25 us, whose bytes alone take 14 at a copy's rate); for many by reading the base and
+// writing the result (6007 tokens, 3584 x 37888: 222 us, of them 210 in the second product at
+// 4.4 TB/s).
 
 #include <hip/hip_runtime.h>
 

@@ -328,7 +328,7 @@ constexpr int kTogether = 4;  // vectors per thread and round
 struct Queue {
   u32x4 raw[kTogether * kThreads];
   uint16_t place[kQueue];
-  int32_t length;
+  int32_t length[2];  // of even and of odd rounds
 };
 
 // ------------------------------------------------------------------------------ first pass
@@ -504,11 +504,13 @@ __device__ __forceinline__ void push_visit(bool wanted, int32_t tile, int32_t* v
 
 // Reads the tiles visit[0 .. visits), four slots per thread at a time and the next four in flight,
 // and calls token(value, index) for every token that is at least `from` (not -inf), by whole waves:
-// what a round finds is queued first.  A wave that wants at least half of its values calls
-// whole(values, mask, slot) for its slots instead: a queue of 4096 takes a workgroup's 32768 values
-// in eight turns (274 x 32000 bf16, nearly flat: the histogram pass 34 us, with the queue alone 61;
-// 200 x 50257 with few tokens wanted: 23 us either way, 25 where a quarter is enough).  One
-// workgroup; queue.length is 0 before and after.
+// what a round finds is queued first, as places in its vectors (values and indices, found by a test
+// per bit: 200 x 50257, the histogram pass 23 us and the gathering 18 instead of 20 and 16).  A wave
+// that wants at least half of its values calls whole(values, mask, slot) for its slots instead
+// (274 x 32000 bf16, nearly flat: the histogram pass 34 us, with the queue alone 61; with a quarter
+// instead of half, 200 x 50257 took 25 us instead of 23).  One
+// workgroup; queue.length is 0 before and after.  Rounds count in two lengths by turns: a wave that
+// leaves a round where nothing was found may count in the next before others have read this one's.
 template <int DT, typename Token, typename Whole>
 __device__ __forceinline__ void read_tiles(const Row<DT>& row, const Tiles<DT>& tiles,
                                            const int32_t* visit, int32_t visits, float from,
@@ -525,7 +527,9 @@ __device__ __forceinline__ void read_tiles(const Row<DT>& row, const Tiles<DT>& 
   u32x4 raw[kTogether];
 #pragma unroll
   for (int u = 0; u < kTogether; ++u) raw[u] = row.request(slot_of(u * kThreads + (int32_t)threadIdx.x));
+  int32_t round = 0;
   for (int32_t i0 = 0; i0 < items; i0 += kTogether * kThreads) {
+    int32_t* length = &queue.length[round++ & 1];
     uint32_t hits = 0;  // one bit per value
 #pragma unroll
     for (int u = 0; u < kTogether; ++u) {
@@ -561,7 +565,7 @@ __device__ __forceinline__ void read_tiles(const Row<DT>& row, const Tiles<DT>& 
     for (int32_t found = kQueue + 1; found > kQueue;) {
       if (all > 0) {
         int32_t at = 0;
-        if (lane == 63) at = atomicAdd(&queue.length, (int32_t)all);
+        if (lane == 63) at = atomicAdd(length, (int32_t)all);
         at = (int32_t)last_lane((uint32_t)at) + (int32_t)(incl - (uint32_t)__popc(hits));
         while (hits && at < kQueue) {
           const int32_t b = __ffs((int)hits) - 1;
@@ -571,7 +575,7 @@ __device__ __forceinline__ void read_tiles(const Row<DT>& row, const Tiles<DT>& 
         }
       }
       lds_barrier();
-      found = queue.length;
+      found = *length;
       if (found == 0) break;
       const int32_t queued = found < kQueue ? found : kQueue;
       for (int32_t i = threadIdx.x; i < queued; i += kThreads) {
@@ -586,7 +590,7 @@ __device__ __forceinline__ void read_tiles(const Row<DT>& row, const Tiles<DT>& 
         all = last_lane(incl);
       }
       lds_barrier();
-      if (threadIdx.x == 0) queue.length = 0;
+      if (threadIdx.x == 0) *length = 0;
       lds_barrier();
     }
   }
@@ -712,7 +716,7 @@ __global__ __launch_bounds__(kThreads) void bins_kernel(SampleArgs a) {
   const float tile_max = t < per && tile < tiles.count ? tiles.max_of(a, r, tile) : -INFINITY;
   const Chunk chunk = own_chunk(a, r);
   for (int32_t b = t; b < 2 * kBins; b += kThreads) s.mass[b] = 0;
-  if (t == 0) s.visits = s.queue.length = 0;
+  if (t == 0) s.visits = s.queue.length[0] = s.queue.length[1] = 0;
   const float top = row_max(chunk, s.wave_max);
   if (top == -INFINITY) return;
   uint64_t mass, total;
@@ -1595,7 +1599,7 @@ __global__ __launch_bounds__(kThreads) void gather_kernel(SampleArgs a) {
     bin = least_bin = nucleus_bin(q, total, s.bin_mass, s, before, binned);
   }
   const float from = bin_from(bin, top);
-  if (t == 0) s.queue.length = 0;
+  if (t < 2) s.queue.length[t] = 0;
   push_visit(tile_max >= from && tile_max > -INFINITY, tile0 + t, s.visit, &s.visits);
   __syncthreads();
   // The mass that a token adds to its tile, or its place in the list.
@@ -1647,9 +1651,9 @@ __global__ __launch_bounds__(kThreads) void gather_kernel(SampleArgs a) {
 // per bin, which gives it exactly (32 x 50257 fp32, top-k 1000: 28.6 us; by the digits 88).  Tiles
 // whose maximum shows that they hold no token of the list or before it are not read.
 //
-// Bound by its steps' latency: 32 x 152064 bf16 with all filters 14.7 us, of those 1.7 for the
-// maximum, 1.7 for the bin, 4 for reading 50 tiles, 2.6 for the order and cut and 2 for the choice;
-// a row without a filter 6.
+// Bound by its steps' latency: 32 x 152064 bf16 with all filters 13 us, of those 1.7 for the maximum,
+// 1.7 for the bin, 3.2 for reading 50 tiles, 2.6 for the order and cut and 1.5 for the choice; a row
+// without a filter 6.
 template <int DT>
 __global__ __launch_bounds__(kThreads) void row_kernel(SampleArgs a) {
   __shared__ RowShared s;
