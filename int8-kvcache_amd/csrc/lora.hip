@@ -727,6 +727,17 @@ bool rows16(const void* p, int64_t stride) {
   return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && stride % 8 == 0;
 }
 
+// Whether the first pn and qn columns of two matrices' rows share memory (rows of different strides:
+// whether the matrices' extents do).
+bool rows_overlap(const void* p, int64_t ps, int64_t pn, const void* q, int64_t qs, int64_t qn,
+                  int64_t rows) {
+  const int64_t at = (int64_t)(reinterpret_cast<intptr_t>(q) - reinterpret_cast<intptr_t>(p)) / 2;
+  if (at >= (rows - 1) * ps + pn || at + (rows - 1) * qs + qn <= 0) return false;
+  if (rows == 1 || ps != qs) return true;
+  const int64_t column = (at % ps + ps) % ps;
+  return column < pn || column + qn > ps;
+}
+
 // Parts of k.  Tiles of 16 tokens: about four workgroups of four waves per compute unit (32 tokens
 // on 24 adapters, the four projections of a layer: 35 us with 12-16 parts, 37 with 8, 56 with 2).
 // Tiles of 64: eight waves, as many workgroups as run at a time, nearly two per unit up to rank 32
@@ -913,6 +924,10 @@ extern "C" int int8kv_lora_add(const void* base, int64_t base_row_stride, const 
   if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 ||
       workspace_bytes < int8kv_lora_workspace_bytes(tokens, num_adapters, k, rank))
     return INT8KV_E_WORKSPACE;
+  const bool in_place = out == base && out_row_stride == base_row_stride;
+  if ((!in_place && rows_overlap(out, out_row_stride, n, base, base_row_stride, n, tokens)) ||
+      rows_overlap(out, out_row_stride, n, x, x_row_stride, k, tokens))
+    return INT8KV_E_STRIDE;
   LoraArgs a;
   a.base = static_cast<const uint16_t*>(base);
   a.base_stride = base_row_stride;

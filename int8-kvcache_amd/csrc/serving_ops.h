@@ -81,7 +81,8 @@ int int8kv_lora_plan(const void* adapter_ids, int ids_dtype, int64_t tokens, int
 /*
  * The product, with the plan of the same tokens and num_adapters.  All matrices bf16 with unit
  * inner strides and 16-byte aligned rows: x [tokens, k], base and out [tokens, n] (out may be
- * base itself, and must not otherwise overlap the inputs), lora_a [num_adapters, rank, k] and
+ * base itself, and must not otherwise overlap the inputs: rows that overlap base's or x's give
+ * INT8KV_E_STRIDE), lora_a [num_adapters, rank, k] and
  * lora_b [num_adapters, n, rank] (strides of the adapters and of the rows).  scales: fp32
  * [num_adapters], or NULL for 1.  k, n and rank multiples of 8, rank at most 128, k and n at most
  * 2^20.  workspace: int8kv_lora_workspace_bytes(...) bytes, 16-byte aligned, no initialisation

@@ -250,3 +250,21 @@ def test_whole_tiles_and_quarters(cuda, tokens, k, n, rank, adapters):
     d["x"][none] = float("nan")
     out = add(d, out=d["base"])
     assert out.data_ptr() == d["base"].data_ptr() and torch.equal(out, want)
+
+
+def test_out_beside_x_in_the_same_rows(cuda):
+    """Columns of one buffer: out beside x is fine, out over x or over base's other rows is refused."""
+    d = inputs(cuda, 21, 264, 136, 16, 3, seed=14)
+    want = add(d)
+    packed = torch.zeros(21, 400, dtype=torch.bfloat16, device=cuda)
+    packed[:, :264] = d["x"]
+    plan = int8kv.lora_plan(d["ids"], 3)
+    rest = dict(scales=d["scales"])
+    got = int8kv.lora_add(d["base"], packed[:, :264], d["a"], d["b"], plan, out=packed[:, 264:], **rest)
+    assert torch.equal(got, want) and torch.equal(packed[:, :264], d["x"])
+    wide = torch.zeros(22, 136, dtype=torch.bfloat16, device=cuda)
+    for base, x, out in ((d["base"], packed[:, :264], packed[:, 128:264]), (wide[:21], d["x"], wide[1:])):
+        with pytest.raises(_lib.Int8KVError, match="STRIDE"):
+            int8kv.lora_add(base, x, d["a"], d["b"], plan, out=out, **rest)
+        with _ext.use_ctypes(), pytest.raises(_lib.Int8KVError, match="STRIDE"):
+            int8kv.lora_add(base, x, d["a"], d["b"], plan, out=out, **rest)

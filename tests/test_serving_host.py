@@ -88,6 +88,24 @@ def test_lora_refusals(lib):
     assert lib.int8kv_lora_workspace_bytes(4, 3, 20, 8) == 0
 
 
+def test_lora_outputs_over_its_inputs_are_refused(lib):
+    """Rows of out that share memory with x, or with base otherwise than in place."""
+    two = ctypes.c_int64 * 2
+    far = P + (1 << 20)
+
+    def call(base, bs, x, xs, out, os, tokens=4, n=64):
+        return lib.int8kv_lora_add(base, bs, x, tokens, 32, xs, P, two(8 * 32, 32), P, two(64 * 8, 8), 3, 8,
+                                   n, None, P, 1 << 20, out, os, P, 1 << 20, None)
+
+    assert call(far, 64, P, 32, P, 64) == -4  # x itself
+    assert call(far, 64, P, 64, P, 64) == -4
+    assert call(P, 64, far, 32, P + 128, 64) == -4  # base's next row
+    assert call(P, 64, far, 32, P, 128) == -4  # base in other rows
+    assert call(P, 256, far, 32, P + 2 * 56, 256) == -4  # columns 56 .. 119 over 0 .. 63
+    assert call(P, 256, far, 32, P - 2 * 56, 256) == -4
+    assert call(P, 64, far, 32, P + 2 * 56, 64, tokens=1) == -4
+
+
 def test_sample_refusals(lib):
     def call(**o):
         a = dict(logits=P, dt=2, rows=4, vocab=100, rs=100, u=P, t=None, k=None, p=None, m=None,
